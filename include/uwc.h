@@ -414,6 +414,56 @@ int uwc_sha_row_leaves(const uint32_t* rows, int64_t nrows, int row_words, uint3
 int uwc_sha_merkle_roots(const uint32_t* leaves, int ntrees, int n, uint32_t* scratch, int64_t scratch_words,
                          uint32_t* roots, hipStream_t stream);
 
+/* ======================================================================== the key/value cache
+ * Paged 8-bit keys and values, and the attention that reads them. No counterpart in the reference
+ * (its DetQwen3.generate_greedy keeps whole fp32 rows, runtime/detrt/qwen3.py:296-334).
+ *
+ * One layer's cache: k int8 (pages, Hkv, page, hd); v int8 (pages, Hkv, hd, page), tokens innermost; ks, vs
+ * fp32 (pages, Hkv), the scale of a page's keys and values of one head. page is 16, 32, 64 or 128, hd 32,
+ * 64 or 128; k and v 16-byte aligned. Token p of sequence b lies in slot p % page of page
+ * table[b * table_stride + p / page]; a row of the table has `width` entries, those past a sequence's pages
+ * are not read.
+ * Packed rows: sequence b's new tokens are rows cu[b] .. cu[b + 1] - 1 (cu int32, B + 1, cu[0] = 0); cu NULL
+ * means one row each (T = B). Rows from cu[B] on belong to no sequence: their outputs are zeros.
+ * 16-bit rows are UWC_KV_BF16 or UWC_KV_FP16. Device-side numbers cannot be refused by a return value: a
+ * page that is needed but outside [0, pages) or past the table's width, or a position past the rotation
+ * tables, makes the rows that need it NaN, and nothing outside the buffers is read or written. */
+#define UWC_KV_BF16 0
+#define UWC_KV_FP16 1
+
+/* The new tokens' heads into the cache and q out. qkv T rows (qkv_stride elements apart, 16-byte aligned)
+ * of H q heads, Hkv k heads, Hkv v heads; ctx[b] tokens of sequence b are cached already. q and k heads:
+ * x / sqrt(mean(x^2) + eps) * w where q_norm / k_norm (fp32, hd) is given, then x cos + (-hi, lo)(x) sin
+ * with row p of the tables cosb, sinb (fp32, positions x hd). q (T, H, hd) in qkv's type. Keys, values:
+ * z = clamp(rint(x / s), -127, 127) with s = max(max|x| over the page's new tokens, 1e-8) / 127, at least
+ * the old scale where the page holds older tokens, which are rounded again, rint(z old / s), if s grew. Slots
+ * past a sequence's last token hold nothing defined. No two sequences' new tokens may share a page. */
+int uwc_kv_append(const void* qkv, int64_t qkv_stride, int dtype, int T, int B, const int32_t* cu, const int32_t* ctx,
+                  const int32_t* table, int64_t table_stride, int width, const float* cosb, const float* sinb,
+                  int positions, const float* q_norm, const float* k_norm, float eps, int H, int Hkv, int hd, int page,
+                  int64_t pages, int8_t* k, int8_t* v, float* ks, float* vs, void* q, hipStream_t stream);
+
+/* o (T, H, hd) = causal attention of q (T tokens, q_stride elements apart, H heads of hd) over the cache:
+ * sequence b has lens[b] tokens in it, its queries are the last of them. window > 0: a query at position p
+ * sees keys above p - window, and those below `sinks`. Scores are scaled by `scale`. Rows that see nothing
+ * are zeros. max_new and max_len (0: unknown) bound the sequences' new tokens and lengths: they choose how
+ * the work is split, and results are right for any. scratch: uwc_kv_attend_scratch_bytes bytes, 16-byte
+ * aligned, no contents kept between calls (may be NULL when that is 0). Sums and softmax statistics are fp32,
+ * probabilities are rounded to fp16 for the product with the values. */
+uint64_t uwc_kv_attend_scratch_bytes(int T, int B, int packed, int H, int Hkv, int hd, int max_new, int max_len,
+                                     int window, int sinks);
+int uwc_kv_attend(const int8_t* k, const int8_t* v, const float* ks, const float* vs, int64_t pages, int page, int Hkv,
+                  int hd, const void* q, int64_t q_stride, int dtype, int T, int H, const int32_t* table,
+                  int64_t table_stride, int width, const int32_t* lens, const int32_t* cu, int B, int max_new,
+                  int max_len, int window, int sinks, float scale, void* scratch, uint64_t scratch_bytes, void* o,
+                  hipStream_t stream);
+
+/* Tokens start[b] .. start[b] + cu[b + 1] - cu[b] - 1 of every sequence as values, z s rounded once:
+ * ko, vo (rows, Hkv, hd). Rows from cu[B] on are not written. */
+int uwc_kv_read(const int8_t* k, const int8_t* v, const float* ks, const float* vs, int64_t pages, int page, int Hkv,
+                int hd, const int32_t* table, int64_t table_stride, int width, const int32_t* start, const int32_t* cu,
+                int B, int rows, int dtype, void* ko, void* vo, hipStream_t stream);
+
 /* Measurement aid (no reference counterpart): iters x 8 v_mfma_i32_32x32x32_i8 per wave in a
  * register-only loop, 8 waves on every CU, with constant (random_operands = 0) or seeded random
  * operands; each MFMA is 65,536 int8 ops. Timing it gives the part's sustained int8 MFMA rate,

@@ -70,10 +70,17 @@ SIGNATURES = {
     "uwc_sha_row_leaves": [vp, i64, i32, vp, i64, u32, u32, u32, vp, vp, vp],
     "uwc_sha_merkle_roots": [vp, i32, i32, vp, i64, vp, vp],
     "uwc_det_elementwise": [i32, vp, vp, vp, i64, vp],
+    "uwc_kv_append": [vp, i64, i32, i32, i32, vp, vp, vp, i64, i32, vp, vp, i32, vp, vp, f32, i32, i32, i32, i32, i64, vp, vp, vp,
+                      vp, vp, vp],
+    "uwc_kv_attend_scratch_bytes": [i32, i32, i32, i32, i32, i32, i32, i32, i32, i32],
+    "uwc_kv_attend": [vp, vp, vp, vp, i64, i32, i32, i32, vp, i64, i32, i32, i32, vp, i64, i32, vp, vp, i32, i32, i32, i32, i32,
+                      f32, vp, u64, vp, vp],
+    "uwc_kv_read": [vp, vp, vp, vp, i64, i32, i32, i32, vp, i64, i32, vp, vp, i32, i32, i32, vp, vp, vp],
     "uwc_mfma_rate_probe": [i32, i32, vp, i64, vp],
 }
 _RESTYPE = {"uwc_last_error": ctypes.c_char_p, "uwc_header_sha": ctypes.c_char_p,
-            "uwc_attention_scratch_bytes": ctypes.c_uint64, "uwc_decoder_layer_scratch_bytes": ctypes.c_uint64}
+            "uwc_attention_scratch_bytes": ctypes.c_uint64, "uwc_decoder_layer_scratch_bytes": ctypes.c_uint64,
+            "uwc_kv_attend_scratch_bytes": ctypes.c_uint64}
 
 _LIB = None
 
