@@ -20,6 +20,8 @@
 //
 // The running maximum m only moves when some row's new maximum exceeds it by 2^8 or more (w then stays below
 // 2^9, far inside fp16), so that most tiles neither exchange maxima between lanes nor rescale O.
+#include <type_traits>
+
 #include "uwc_kv.h"
 
 namespace {
@@ -74,9 +76,10 @@ struct Span {
   int st, lt, n;
   __device__ __forceinline__ int tile(int t) const { return t < st ? t : lt + t - st; }
 };
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ Span span_of(const AttendArgs& a, int p_lo, int p_hi) {
   Span s;
-  s.p_lo = p_lo, s.p_hi = p_hi;
+  s.p_lo = p_lo = uniform(p_lo), s.p_hi = p_hi = uniform(p_hi);
   s.lo = a.window && p_lo >= a.window ? p_lo - a.window + 1 : 0;
   s.lt = s.lo >> 6;
   const int first = (a.sinks + 63) >> 6;
@@ -120,14 +123,19 @@ __device__ __forceinline__ bool unit_of(const AttendArgs& a, int& u, int M, Unit
     b = u / per, j = u % per;
     x.row0 = b;
   }
-  x.b = b, x.r0 = j * M, x.rows = kv_new(a.rows, b) * a.G, x.len = a.lens[b];
+  x.b = uniform(b), x.r0 = uniform(j * M), x.rows = uniform(kv_new(a.rows, b) * a.G), x.len = uniform(a.lens[b]);
+  x.row0 = uniform(x.row0);
   return true;
 }
 
-// The packed row and head of row r of a unit as an index into (T, H), or -1.
-__device__ __forceinline__ long out_row(const AttendArgs& a, const Unit& x, int r, int h) {
-  const int t = x.row0 + r / a.G;
-  return r < x.rows && t >= 0 && t < a.rows.T ? (long)t * a.H + h * a.G + r % a.G : -1;
+// Row r of a unit: its packed row t (-1 outside) and head; row = t H + head.
+struct Place {
+  int t, head;
+  __device__ __forceinline__ long row(const AttendArgs& a) const { return t < 0 ? -1 : (long)t * a.H + head; }
+};
+__device__ __forceinline__ Place place_of(const AttendArgs& a, const Unit& x, int r, int h) {
+  const int i = r / a.G, t = x.row0 + i;
+  return Place{r < x.rows && t >= 0 && t < a.rows.T ? t : -1, h * a.G + r - i * a.G};
 }
 
 template <class T, int N>
@@ -244,9 +252,9 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(AttendArgs a) {
 #pragma unroll
   for (int rb = 0; rb < RB; rb++) {
     const int r = x.r0 + rb * 16 + m16;
-    const long row = out_row(a, x, r, h);
-    pos[rb] = row < 0 ? -1 : x.pos(a, r);
-    const T* qp = static_cast<const T*>(a.q) + (row < 0 ? 0 : (row / a.H) * a.q_stride + (row % a.H) * HD);
+    const Place at = place_of(a, x, r, h);
+    pos[rb] = at.t < 0 ? -1 : x.pos(a, r);
+    const T* qp = static_cast<const T*>(a.q) + (at.t < 0 ? 0 : at.t * a.q_stride + at.head * HD);
     v8 w[KS];
     u32 top = 0;
 #pragma unroll
@@ -317,9 +325,11 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(AttendArgs a) {
       float e[16], top = -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < 16; i++) e[i] = __builtin_fmaf(s[rb][i >> 2][i & 3], Ak, lv);
-      if (!whole)
+      if (!whole) {
+        asm volatile("" : "+v"(pos[rb]));  // keeps this a branch
 #pragma unroll
         for (int i = 0; i < 16; i++) e[i] = seen(a, pos[rb], kt * 64 + 16 * g + i) ? e[i] : -__builtin_inff();
+      }
 #pragma unroll
       for (int i = 0; i < 16; i++) top = fmaxf(top, e[i]);
       if (__any(top > mr[rb] + KV_SLACK)) {
@@ -374,7 +384,7 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(AttendArgs a) {
     __syncthreads();
     constexpr int N = HD / 16;
     const int ro = tid >> 4, d = (tid & 15) * N, rr = rb * 16 + ro;
-    const long row = out_row(a, x, x.r0 + rr, h);
+    const long row = place_of(a, x, x.r0 + rr, h).row(a);
     if (row >= 0) {
       float y[N], tm = fmaxf(fmaxf(sm[0][rr], sm[1][rr]), fmaxf(sm[2][rr], sm[3][rr])), tl = 0.0f;
 #pragma unroll
@@ -384,6 +394,345 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(AttendArgs a) {
       put<HD, N, T>(a, row, split, d, y, tm, tl);
     }
   }
+}
+
+// ------------------------------------------------------------------ many rows
+// A workgroup of NW waves takes 32 NW rows of one kv head; the keys and values of a 64-key tile are turned into
+// fp16 once per workgroup, in LDS, and every wave multiplies its own 32 rows with them on 32 x 32 x 16 matrix
+// instructions. A step has two halves with a barrier after each: the weights of a tile (VALU: 32 exponentials of 16
+// cycles each and some 130 other instructions per wave, about 1200 cycles), and its product with V and the next tile's
+// scores (32 matrix instructions, 1024 cycles, fed by LDS reads six ahead), between which the next bytes are
+// converted, written to LDS and loaded. With eight waves the two of a SIMD take turns at the halves, a barrier apart.
+//
+// Four waves (two workgroups to a CU) keep two stages of keys and of values: the keys of tile i + 2 are written in
+// the second half of step i, when keys i are done with and keys i + 1 are read; the values of tile i + 1 in the first half of
+// step i, when values i - 1 are done with. Eight waves keep four stages of either, as the waves that are half a
+// step behind still read values i when the others are a half past them, and write tile i + 2 in step i's second half.
+//
+// LDS rows hold 16-byte pieces (8 fp16), piece c of row r at c ^ swz(r), so that the 32 rows of an operand are
+// read without bank conflicts. K's operand row m is key 16 (m >> 4) + 8 (m >> 2 & 1) + 4 (m >> 3 & 1) +
+// (m & 3) of its 32: the scores of lane half hf are then keys 16 n + 8 hf + i, the 8 k slots of V's product n.
+//
+// Measured: 4096 tokens over 32768, 16 heads of 128, 985 us = 1048 TFLOP/s at a clock that the load drives down to
+// about 1.85 GHz (an fp16 product of 16384^3 reaches 1316 here): 3780 cycles for 64 keys of 256 rows, of which the
+// matrix units are busy 2048.
+__device__ __forceinline__ int key_row(int key) { return (key & ~12) | ((key & 4) << 1) | ((key & 8) >> 1); }
+template <int HD>
+__device__ __forceinline__ int k_piece(int r, int c) {  // of rows of HD fp16
+  if (HD == 32) return r * 4 + (c ^ ((r >> 1) & 3));
+  if (HD == 128) c = c >> 1 | (c & 1) << 3;  // the eight lanes that write a row's even pieces hit all banks
+  return r * (HD / 8) + (c ^ ((r ^ (r >> 3 & 3)) & 7));
+}
+__device__ __forceinline__ int v_piece(int r, int c) { return r * 8 + (c ^ ((r ^ (r >> 3 & 3)) & 7)); }
+
+// The weights of one 32-row block for a tile of 64 keys: p the operands of V's products, m the running maximum and
+// l this lane's part of the denominator brought up to date, o rescaled where m moved.
+template <int DB>
+__device__ __forceinline__ void softmax_tile(const AttendArgs& a, f16v s[2], float A, int& pos, bool whole, int key0,
+                                             const float4* meta, f16v* o, float& mr, float& l, h8v p[4]) {
+  // 2^(s Ak + lk - m) is the weight; Ak > 0, so the maximum of s gives that of the exponent
+  float Ak[4], lk[4], rv[4], top = -__builtin_inff();
+#pragma unroll
+  for (int n = 0; n < 4; n++) {
+    const float4 mt = meta[n];
+    Ak[n] = A * mt.x, lk[n] = mt.y, rv[n] = mt.z;
+  }
+  if (!whole) {
+    asm volatile("" : "+v"(pos));  // keeps this a branch
+#pragma unroll
+    for (int n = 0; n < 4; n++) {
+      bool some = false;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const bool y = seen(a, pos, key0 + 16 * n + i);
+        s[n >> 1][8 * (n & 1) + i] = y ? s[n >> 1][8 * (n & 1) + i] : -__builtin_inff();
+        some |= y;
+      }
+      // -inf has to stay -inf, also under a scale of 0, and under any scale of keys this row does not see
+      Ak[n] = !some ? 1.0f : Ak[n] == 0.0f ? 0x1p-126f : Ak[n];
+      lk[n] = some ? lk[n] : 0.0f;
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < 4; n++) {
+    float g = s[n >> 1][8 * (n & 1)];
+#pragma unroll
+    for (int i = 1; i < 8; i++) g = fmaxf(g, s[n >> 1][8 * (n & 1) + i]);
+    top = fmaxf(top, __builtin_fmaf(g, Ak[n], lk[n]));
+  }
+  if (__any(top > mr + KV_SLACK)) {
+    const float to = fmaxf(mr, max_xor32(top));
+    const float f = __builtin_amdgcn_exp2f(mr - to);
+    mr = to;
+    l *= f;
+#pragma unroll
+    for (int db = 0; db < DB; db++) o[db] *= f;
+  }
+#pragma unroll
+  for (int n = 0; n < 4; n++) {
+    const float b = lk[n] - mr;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n >> 1][8 * (n & 1) + i], Ak[n], b));
+      sum += w;
+      p[n][i] = (_Float16)w;
+    }
+    l = sum == 0.0f ? l : __builtin_fmaf(sum, rv[n], l);  // keys nobody sees may have any scale
+  }
+}
+
+typedef h8v __attribute__((address_space(3)))* lds_h8;
+__device__ __forceinline__ u32 lds_addr(const h8v* q) { return (u32)(uintptr_t)(void __attribute__((address_space(3)))*)q; }
+__device__ __forceinline__ void lds_put(u32 a, h8v v) { *(lds_h8)(uintptr_t)a = v; }
+
+// LDS operations done, then everyone's; loads from memory stay on their way
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <int HD, int NW, class T>
+__global__ __launch_bounds__(64 * NW, 2) void kv_attend_many_kernel(AttendArgs a) {
+  typedef typename kv_vec<T>::v8 v8;
+  constexpr bool TURNS = NW == 8;
+  constexpr int M = 32 * NW, NT = 64 * NW, KS = HD / 16, DB = HD / 32, STAGES = TURNS ? 4 : 2;
+  constexpr int ROOM = 64 * HD / 8;  // pieces of fp16 of a tile's keys, and of its values
+  __shared__ __attribute__((aligned(256))) h8v sk[STAGES * ROOM], sv[STAGES * ROOM];
+  __shared__ float4 meta[32][4];  // ks, log2(vs), 1 / vs of a tile's granules
+  __shared__ int ids[32][4];      // their pages
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), hf = lane >> 5, m32 = lane & 31;
+  const int h = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, split = rest % a.splits;
+  int u = a.units - 1 - rest / a.splits;  // the last rows of a sequence see the most keys: first
+  Unit x;
+  if (!unit_of(a, u, M, x)) {
+    zero_rows<HD, T>(a, u, M, h, split);
+    return;
+  }
+
+  const int r = x.r0 + wave * 32 + m32;
+  const Place mine = place_of(a, x, r, h);
+  int pos = mine.t < 0 ? -1 : x.pos(a, r);
+  const T* qp = static_cast<const T*>(a.q) + (mine.t < 0 ? 0 : mine.t * a.q_stride + mine.head * HD);
+
+  const int last_r = x.r0 + M < x.rows ? x.r0 + M - 1 : x.rows - 1;
+  const Span sp = span_of(a, x.pos(a, x.r0), x.pos(a, last_r));
+  const int t0 = split * a.tps, n = uniform((split + 1 == a.splits ? sp.n : min(sp.n, (split + 1) * a.tps)) - t0);
+
+  // The pages and scales of 16 tiles at a time, by the first wave, a lane a granule: the table is read at a step
+  // that starts 16 tiles, the scales some steps later, and when 8 are left both are put into LDS for the next 16.
+  const int* const pages_of = a.table + x.b * a.table_stride;
+  struct Granule {
+    int page;  // -2: nobody looks
+    float ks, vs;
+  };
+  auto load_page = [&](int t, Granule& c) KV_AI {
+    t += lane >> 2;
+    const int key0 = sp.tile(t0 + t) * 64 + 16 * (lane & 3), col = key0 >> a.lp;
+    c.page = -2;
+    if (t < n && any_seen(a, sp, key0, 16)) c.page = col < a.width ? pages_of[col] : -1;
+  };
+  auto load_scales = [&](Granule& c) KV_AI {
+    c.page = c.page < a.pages ? c.page : -1;
+    const long at = (long)max(c.page, 0) * a.Hkv + h;
+    c.ks = a.ks[at], c.vs = a.vs[at];
+  };
+  auto put_granule = [&](int t, const Granule& c) KV_AI {
+    const float vs = fmaxf(c.vs, 0x1p-90f);
+    const float4 m{c.page < 0 ? kv_nan() : c.ks, c.vs != c.vs ? c.vs : __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs), 0};
+    meta[(t + (lane >> 2)) & 31][lane & 3] = c.page == -2 ? float4{0, 0, 0, 0} : m;
+    ids[(t + (lane >> 2)) & 31][lane & 3] = c.page;
+  };
+
+  Granule next{-2, 0, 0};
+  if (wave == 0) {
+    load_page(0, next);
+    next.page = next.page < a.pages ? next.page : -1;
+    ids[lane >> 2][lane & 3] = next.page;
+  }
+
+  // The 16-byte pieces of a tile's keys, then those of its values, dealt to the threads; a wave's k-th
+  // pieces are all of one kind.
+  constexpr int PIECES = 64 * HD / 16, PER = 2 * PIECES > NT ? 2 * PIECES / NT : 1;
+  const int mask = (1 << a.lp) - 1;
+  const bool busy = 2 * PIECES >= NT || tid < 2 * PIECES;
+  const u32 page_bytes = ((u32)a.Hkv << a.lp) * HD;
+  const i8 *kh = a.k + ((long)h << a.lp) * HD, *vh = a.v + ((long)h << a.lp) * HD;
+  u32 poff[PER], dst[PER];  // where a piece lies in a page, the tile's first key apart, and its first half in LDS
+  int gran[PER];            // its granule
+  auto of_values = [&](int k) KV_AI { return PER > 1 ? k >= PER / 2 : uniform(tid >= PIECES); };
+#pragma unroll
+  for (int k = 0; k < PER; k++) {
+    const int p = (tid + k * NT) % PIECES, key = p / (HD / 16), c = p % (HD / 16), d = p >> 2, tg = p & 3;
+    const bool values = of_values(k);
+    poff[k] = values ? (u32)((d << a.lp) + ((16 * tg) & mask)) : (u32)((key & mask) * HD + 16 * c);
+    gran[k] = values ? tg : key >> 4;
+    dst[k] = lds_addr(values ? sv + v_piece(d, 2 * tg) : sk + k_piece<HD>(key_row(key), 2 * c));
+  }
+
+  h8v q[KS];
+  float A = 0.0f;
+  f16v o[DB];
+  float mr = KV_LOWEST, l = 0.0f;
+#pragma unroll
+  for (int db = 0; db < DB; db++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[db][i] = 0.0f;
+  if (n > 0) {
+    u4v st[PER];
+    int idp[PER];  // the pages of the next pieces to be loaded
+    h8v p[4];
+    f16v s[2];
+    auto load_id = [&](int i, int k) KV_AI { idp[k] = ids[i & 31][gran[k]]; };
+    auto load_piece = [&](int i, int k) KV_AI {
+      const int off = (sp.tile(t0 + i) * 64) & mask;  // pages of 64 and fewer start with a tile
+      st[k] = *reinterpret_cast<const u4v*>((of_values(k) ? vh + off : kh + off * HD) + ((u64)(u32)max(idp[k], 0) * page_bytes + poff[k]));
+    };
+    auto half_to_lds = [&](int i, int k, int half) KV_AI {  // the second half lies 8 pieces on in the keys' rows of 16, else 1
+      const u32 to = half ? dst[k] ^ (HD == 128 && !of_values(k) ? 128 : 16) : dst[k];
+      lds_put(to + i % STAGES * ROOM * 16, to_half8(st[k][2 * half], st[k][2 * half + 1]));
+    };
+    auto k_frag = [&](int stage, int kb, int ks) KV_AI {
+      return sk[stage * ROOM + 32 * kb * (HD / 8) + k_piece<HD>(m32, 2 * ks + hf)];
+    };
+    auto v_frag = [&](int stage, int db, int g) KV_AI {
+      return sv[stage * ROOM + 32 * db * 8 + v_piece(m32, 2 * g + hf)];
+    };
+    // products 0 .. 4 DB - 1 are those of a tile's weights with its values, the rest the next tile's scores
+    constexpr int NV = 4 * DB, NP = NV + 2 * KS, PRE = 6;
+    auto frag = [&](int S, int k) KV_AI {
+      return k < NV ? v_frag(S % STAGES, k % DB, k / DB) : k_frag((S + 1) % STAGES, (k - NV) & 1, (k - NV) >> 1);
+    };
+    auto product = [&](int k, h8v f) KV_AI {
+      if (k < NV) {
+        o[k % DB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, p[k / DB], o[k % DB], 0, 0, 0);
+      } else {
+        const int kb = (k - NV) & 1, ks = (k - NV) >> 1;
+        if (ks == 0)
+#pragma unroll
+          for (int e = 0; e < 16; e++) s[kb][e] = 0.0f;
+        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, q[ks], s[kb], 0, 0, 0);
+      }
+    };
+
+    // steps 0 and 1 are staged here (four waves: of the values step 0), the next one's bytes are on their way
+    u4v st0[PER], st1[PER];
+    lds_barrier();
+    if (busy) {
+#pragma unroll
+      for (int i = 0; i < 3; i++)
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+          load_id(i, k), load_piece(i, k);
+          if (i == 0) st0[k] = st[k];
+          if (i == 1) st1[k] = st[k];
+        }
+    }
+    if (wave == 0) load_scales(next);
+    {
+      v8 w[KS];
+      u32 top = 0;
+#pragma unroll
+      for (int s = 0; s < KS; s++) {
+        w[s] = *reinterpret_cast<const v8*>(qp + 16 * s + 8 * hf);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const u32 bits = __float_as_uint((float)w[s][i]) & 0x7fffffffu;
+          top = bits > top ? bits : top;
+        }
+      }
+      const u32 other = (u32)__shfl_xor((int)top, 32, 64);
+      top = other > top ? other : top;
+      const int e = q_shift(top);
+      A = __builtin_amdgcn_ldexpf(a.c, -e);
+#pragma unroll
+      for (int s = 0; s < KS; s++) q[s] = scaled_q<T>(w[s], e);
+    }
+    if (busy) {
+#pragma unroll
+      for (int k = 0; k < PER; k++) {
+        const u4v st2 = st[k];
+        const bool one = !TURNS && of_values(k);
+        st[k] = st0[k], half_to_lds(0, k, 0), half_to_lds(0, k, 1);
+        if (!one) st[k] = st1[k], half_to_lds(1, k, 0), half_to_lds(1, k, 1);
+        st[k] = one ? st1[k] : st2;
+        load_id(one ? 2 : 3, k);
+      }
+    }
+    if (wave == 0) put_granule(0, next);
+    lds_barrier();
+
+    // A step: a tile's weights; then its product with V, and the next tile's scores.
+    auto step = [&](int i, auto slot_) KV_AI {
+      constexpr int S = decltype(slot_)::value;
+      if (wave == 0) {
+        if (S == 0 && i % 16 == 0) load_page(i + 16, next);
+        if (S == 0 && i % 16 == 4) load_scales(next);
+        if (S == 0 && i % 16 == 8) put_granule(i + 8, next);
+      }
+      if (!TURNS)
+#pragma unroll
+        for (int k = 0; k < PER; k++)
+          if (of_values(k)) {
+            half_to_lds(S + 1, k, 0), half_to_lds(S + 1, k, 1);
+            load_piece(i + 2, k);
+          }
+      const int key0 = sp.tile(t0 + i) * 64;
+      softmax_tile<DB>(a, s, A, pos, all_seen(a, sp, key0, 64), key0 + 8 * hf, meta[i & 31], o, mr, l, p);
+      __builtin_amdgcn_sched_barrier(0);
+      lds_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
+      h8v f[PRE];
+#pragma unroll
+      for (int k = 0; k < PRE; k++) f[k] = frag(S, k);
+      __builtin_amdgcn_sched_barrier(0);
+      // Between the products, a part at a time: step i + 2's pieces into LDS, step i + 3's loads, the pages for the
+      // loads after those (four waves: of the keys; the values' turn is above). What is past the last tile is for nothing.
+      constexpr int MINE = !TURNS && PER > 1 ? PER / 2 : PER, PARTS = 3 * MINE + 1;
+#pragma unroll
+      for (int k = 0; k < NP; k++) {
+        product(k, f[k % PRE]);
+        if (k + PRE < NP) f[k % PRE] = frag(S, k + PRE);
+        if (busy)
+#pragma unroll
+          for (int j = 0; j < PARTS; j++)
+            if (k == (2 * j + 1) * NP / (2 * PARTS + 2)) {
+              if (j == PARTS - 1) {
+#pragma unroll
+                for (int c = 0; c < PER; c++) load_id(!TURNS && of_values(c) ? i + 3 : i + 4, c);
+              } else if (TURNS || !of_values(j / 3)) {
+                if (j % 3 == 2) load_piece(i + 3, j / 3);
+                else half_to_lds(S + 2, j / 3, j % 3);
+              }
+            }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+      lds_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    // The two waves of a SIMD take turns: while one is at its weights the other is at its products.
+    if (TURNS && wave >= 4) lds_barrier();
+#pragma unroll
+    for (int k = NV; k < NP; k++) product(k, frag(STAGES - 1, k));
+    lds_barrier();
+    for (int i = 0; i < n; i += 4) {
+      step(i, std::integral_constant<int, 0>{});
+      if (i + 1 < n) step(i + 1, std::integral_constant<int, 1>{});
+      if (i + 2 < n) step(i + 2, std::integral_constant<int, 2>{});
+      if (i + 3 < n) step(i + 3, std::integral_constant<int, 3>{});
+    }
+    if (TURNS && wave < 4) lds_barrier();
+  }
+  l += __shfl_xor(l, 32, 64);
+  const long row = mine.row(a);
+  if (row < 0) return;
+#pragma unroll
+  for (int db = 0; db < DB; db++)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const float y[4] = {o[db][i], o[db][i + 1], o[db][i + 2], o[db][i + 3]};
+      put<HD, 4, T>(a, row, split, 32 * db + 2 * i + 4 * hf, y, mr, l);
+    }
 }
 
 // The splits' parts of one row: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.
@@ -417,10 +766,11 @@ __global__ __launch_bounds__(256) void kv_attend_join_kernel(AttendArgs a, long 
 }
 
 // ------------------------------------------------------------------ the split of a call
+enum { KV_FEW, KV_MANY4, KV_MANY8 };  // few rows; many, four or eight waves
 struct Plan {
-  int rb;              // 16-row blocks of a tile of rows
-  long units;          // bound on the tiles of rows
-  int splits, tps;     // splits of the keys, tiles of 64 keys of one
+  int form, m;      // the kernel, and the rows of one of its tiles
+  long units;       // bound on the tiles of rows
+  int splits, tps;  // splits of the keys, tiles of 64 keys of one
   uint64_t o_bytes, bytes;
 };
 
@@ -428,9 +778,13 @@ Plan plan_of(int T, int B, bool packed, int H, int Hkv, int hd, int max_new, int
   Plan p;
   const int G = H / Hkv;
   const long rows = (long)(packed ? (max_new > 0 && max_new < T ? max_new : T) : 1) * G;
-  (void)rows;
-  p.rb = 1;
-  const int M = 16 * p.rb;
+  // 256 rows share a tile's conversion where that still fills the CUs, 128 rows leave less idle where not (us, 256 / 128
+  // rows: 4096 tokens over 32768, 2 heads to a kv head of 128, 985 / 1116; ragged prompts up to 777, 60 / 24; 6000 tokens
+  // under a window of 1024, 4 heads of 64, 76 / 59)
+  const bool wide = hd == 128 && !window && (long)T * G / 256 * Hkv >= uwc_cu_count();
+  p.form = rows <= 32 ? KV_FEW : wide ? KV_MANY8 : KV_MANY4;
+  p.m = p.form == KV_FEW ? 16 : p.form == KV_MANY4 ? 128 : 256;
+  const int M = p.m;
   p.units = packed ? ((long)T * G + M - 1) / M + B : (long)B * ((G + M - 1) / M);
   long keys = max_len > 0 ? max_len : 1;
   if (window && (long)window + sinks + M / G + 128 < keys) keys = (long)window + sinks + M / G + 128;
@@ -460,12 +814,13 @@ extern "C" int uwc_kv_attend(const int8_t* k, const int8_t* v, const float* ks, 
                              hipStream_t stream) {
   const char* fn = "uwc_kv_attend";
   if (!k || !v || !ks || !vs) return uwc_fail("%s: null cache", fn);
-  if (pages <= 0 || pages > 0x7fffffff || Hkv <= 0) return uwc_fail("%s: bad pages=%ld Hkv=%d", fn, (long)pages, Hkv);
+  if (pages <= 0 || pages > 0x7fffffff || Hkv <= 0 || Hkv > 65535) return uwc_fail("%s: bad pages=%ld Hkv=%d", fn, (long)pages, Hkv);
   if (page != 16 && page != 32 && page != 64 && page != 128) return uwc_fail("%s: page %d not in {16, 32, 64, 128}", fn, page);
   if (hd != 32 && hd != 64 && hd != 128) return uwc_fail("%s: head_dim %d not in {32, 64, 128}", fn, hd);
   if (dtype != UWC_KV_BF16 && dtype != UWC_KV_FP16) return uwc_fail("%s: unknown dtype %d", fn, dtype);
   if (H <= 0 || H % Hkv) return uwc_fail("%s: H=%d is no multiple of Hkv=%d", fn, H, Hkv);
   if (T < 0 || B < 0 || width < 0 || table_stride < 0) return uwc_fail("%s: bad T=%d B=%d width=%d", fn, T, B, width);
+  if (!(scale > 0.0f) || scale > 3e38f) return uwc_fail("%s: the scale of the scores must be positive", fn);
   if (window < 0 || sinks < 0 || (sinks && !window)) return uwc_fail("%s: bad window=%d sinks=%d", fn, window, sinks);
   if (T == 0 || B == 0) return UWC_OK;
   if (!q || !table || !lens || !o) return uwc_fail("%s: null arguments", fn);
@@ -483,14 +838,21 @@ extern "C" int uwc_kv_attend(const int8_t* k, const int8_t* v, const float* ks, 
                __builtin_ctz((unsigned)page), window, sinks, scale * 1.4426950408889634f, (int)p.units, p.splits, p.tps, o,
                static_cast<float*>(scratch), reinterpret_cast<float2*>(static_cast<char*>(scratch) + p.o_bytes)};
   const dim3 grid((unsigned)blocks), wg(256);
-#define KV_FEW(HD)                                                                                              \
-  do {                                                                                                          \
-    if (dtype == UWC_KV_BF16) hipLaunchKernelGGL((kv_attend_few_kernel<HD, 1, __bf16>), grid, wg, 0, stream, a); \
-    else hipLaunchKernelGGL((kv_attend_few_kernel<HD, 1, _Float16>), grid, wg, 0, stream, a);                   \
+#define KV_GO(KERNEL_BF16, KERNEL_FP16, threads)                                                                  \
+  do {                                                                                                            \
+    if (dtype == UWC_KV_BF16) hipLaunchKernelGGL((KERNEL_BF16), grid, dim3(threads), 0, stream, a);               \
+    else hipLaunchKernelGGL((KERNEL_FP16), grid, dim3(threads), 0, stream, a);                                    \
   } while (0)
-  if (hd == 32) KV_FEW(32);
-  else if (hd == 64) KV_FEW(64);
-  else KV_FEW(128);
+#define KV_MANY(HD, NW) KV_GO((kv_attend_many_kernel<HD, NW, __bf16>), (kv_attend_many_kernel<HD, NW, _Float16>), 64 * NW)
+#define KV_FORMS(HD)                                                                                          \
+  do {                                                                                                        \
+    if (p.form == KV_FEW) KV_GO((kv_attend_few_kernel<HD, 1, __bf16>), (kv_attend_few_kernel<HD, 1, _Float16>), 256); \
+    else if (p.form == KV_MANY4) KV_MANY(HD, 4);                                                            \
+    else KV_MANY(HD, 8);                                                                                      \
+  } while (0)
+  if (hd == 32) KV_FORMS(32);
+  else if (hd == 64) KV_FORMS(64);
+  else KV_FORMS(128);
   if (int st = uwc_launch_status(fn)) return st;
   if (p.splits == 1) return UWC_OK;
 #define KV_JOIN(HD)                                                                                                       \

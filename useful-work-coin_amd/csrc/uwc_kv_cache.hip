@@ -353,7 +353,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
 int check_cache(const char* fn, const void* k, const void* v, const void* ks, const void* vs, long pages, int page, int Hkv,
                 int hd, int dtype) {
   if (!k || !v || !ks || !vs) return uwc_fail("%s: null cache", fn);
-  if (pages <= 0 || pages > 0x7fffffff || Hkv <= 0) return uwc_fail("%s: bad pages=%ld Hkv=%d", fn, pages, Hkv);
+  if (pages <= 0 || pages > 0x7fffffff || Hkv <= 0 || Hkv > 65535) return uwc_fail("%s: bad pages=%ld Hkv=%d", fn, pages, Hkv);
   if (page != 16 && page != 32 && page != 64 && page != 128) return uwc_fail("%s: page %d not in {16, 32, 64, 128}", fn, page);
   if (hd != 32 && hd != 64 && hd != 128) return uwc_fail("%s: head_dim %d not in {32, 64, 128}", fn, hd);
   if (dtype != UWC_KV_BF16 && dtype != UWC_KV_FP16) return uwc_fail("%s: unknown dtype %d", fn, dtype);
