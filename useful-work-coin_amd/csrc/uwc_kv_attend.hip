@@ -743,10 +743,13 @@ __global__ __launch_bounds__(256) void kv_attend_join_kernel(AttendArgs a, long 
   __shared__ float sl[GROUPS];
   const int tid = threadIdx.x, c = tid % LPR, grp = tid / LPR;
   const long R = (long)a.rows.T * a.H, row = row_base + blockIdx.x;
-  float m = KV_LOWEST;
-  for (int s = 0; s < a.splits; s++) m = fmaxf(m, a.ml[s * R + row].x);
+  float m = KV_LOWEST;  // every wave looks at all parts' maxima, a lane each
+  for (int s = tid & 63; s < a.splits; s += 64) m = fmaxf(m, a.ml[s * R + row].x);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
   f32x4 o{0, 0, 0, 0};
   float l = 0.0f;
+#pragma unroll 4
   for (int s = grp; s < a.splits; s += GROUPS) {
     const float2 v = a.ml[s * R + row];
     const float f = __builtin_amdgcn_exp2f(v.x - m);
@@ -788,10 +791,15 @@ Plan plan_of(int T, int B, bool packed, int H, int Hkv, int hd, int max_new, int
   p.units = packed ? ((long)T * G + M - 1) / M + B : (long)B * ((G + M - 1) / M);
   long keys = max_len > 0 ? max_len : 1;
   if (window && (long)window + sinks + M / G + 128 < keys) keys = (long)window + sinks + M / G + 128;
-  const long tiles = (keys + 63) / 64, want = 2L * uwc_cu_count() / (p.units * Hkv);
-  long splits = want < 1 ? 1 : want;
+  const long tiles = (keys + 63) / 64;
+  // Few rows: two workgroups fit a CU. Where sequences and heads alone fill the CUs, their lengths may differ and the
+  // keys are cut into pieces that make four rounds' worth (48 sequences of 1500 to 12000 tokens, 8 kv heads: 153 us;
+  // two per CU 204, none cut 166); where they do not, into as many as fit at once (one of 131072: 55 us with one or two
+  // per CU, 59 with four, 68 with eight), down to one tile a wave (one of 2500: 9.7 us; two tiles 11.8, four 15.6).
+  const long wgs = p.units * Hkv, cus = uwc_cu_count();
+  long splits = p.form == KV_FEW ? wgs >= cus ? (4 * cus + wgs - 1) / wgs : 2 * cus / wgs : 2 * cus / wgs;
   if (splits > (tiles + 3) / 4) splits = (tiles + 3) / 4;
-  if (splits > 1024) splits = 1024;
+  if (splits < 1) splits = 1;
   p.tps = (int)((tiles + splits - 1) / splits);
   p.splits = (int)((tiles + p.tps - 1) / p.tps);
   p.o_bytes = p.splits > 1 ? (uint64_t)p.splits * T * H * hd * 4 : 0;
