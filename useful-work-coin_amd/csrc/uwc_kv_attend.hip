@@ -735,41 +735,49 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attend_many_kernel(AttendArgs a
     }
 }
 
-// The splits' parts of one row: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.
-template <int HD, class T>
-__global__ __launch_bounds__(256) void kv_attend_join_kernel(AttendArgs a, long row_base) {
-  constexpr int LPR = HD / 4, GROUPS = 256 / LPR;  // lanes of 4 dims per part; parts read at once
+// The splits' parts of a row: o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s. Few parts: hd / 4 lanes a row, its
+// parts in turn. Many: a workgroup a row, its groups of hd / 4 lanes every GROUPS-th part each, joined in LDS.
+template <int HD, bool MANY, class T>
+__global__ __launch_bounds__(256) void kv_attend_join_kernel(AttendArgs a, long row_base, long row_end) {
+  constexpr int LPR = HD / 4, GROUPS = 256 / LPR;
   __shared__ f32x4 so[GROUPS][LPR];
   __shared__ float sl[GROUPS];
   const int tid = threadIdx.x, c = tid % LPR, grp = tid / LPR;
-  const long R = (long)a.rows.T * a.H, row = row_base + blockIdx.x;
-  float m = KV_LOWEST;  // every wave looks at all parts' maxima, a lane each
-  for (int s = tid & 63; s < a.splits; s += 64) m = fmaxf(m, a.ml[s * R + row].x);
+  const long R = (long)a.rows.T * a.H, row = row_base + (MANY ? (long)blockIdx.x : (long)blockIdx.x * GROUPS + grp);
+  if (!MANY && row >= row_end) return;
+  float m = KV_LOWEST;
+  if constexpr (MANY) {  // every wave looks at all parts' maxima, a lane each
+    for (int s = tid & 63; s < a.splits; s += 64) m = fmaxf(m, a.ml[s * R + row].x);
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+  } else {
+    for (int s = 0; s < a.splits; s++) m = fmaxf(m, a.ml[s * R + row].x);
+  }
   f32x4 o{0, 0, 0, 0};
   float l = 0.0f;
 #pragma unroll 4
-  for (int s = grp; s < a.splits; s += GROUPS) {
+  for (int s = MANY ? grp : 0; s < a.splits; s += MANY ? GROUPS : 1) {
     const float2 v = a.ml[s * R + row];
     const float f = __builtin_amdgcn_exp2f(v.x - m);
     l = __builtin_fmaf(v.y, f, l);
     o += *reinterpret_cast<const f32x4*>(a.po + (s * R + row) * HD + 4 * c) * f;
   }
-  so[grp][c] = o;
-  if (c == 0) sl[grp] = l;
-  __syncthreads();
-  if (tid >= LPR) return;
-  l = 0.0f, o = f32x4{0, 0, 0, 0};
+  if constexpr (MANY) {
+    so[grp][c] = o;
+    if (c == 0) sl[grp] = l;
+    __syncthreads();
+    if (tid >= LPR) return;
+    l = 0.0f, o = f32x4{0, 0, 0, 0};
 #pragma unroll
-  for (int i = 0; i < GROUPS; i++) l += sl[i], o += so[i][c];
+    for (int i = 0; i < GROUPS; i++) l += sl[i], o += so[i][c];
+  }
   const float r = l == 0.0f ? 0.0f : 1.0f / l;
   float y[4] = {o[0] * r, o[1] * r, o[2] * r, o[3] * r};
   store_row<T, 4>(static_cast<T*>(a.o) + row * HD + 4 * c, y);
 }
 
 // ------------------------------------------------------------------ the split of a call
-enum { KV_FEW, KV_MANY4, KV_MANY8 };  // few rows; many, four or eight waves
+enum { KV_FEW1, KV_FEW2, KV_MANY4, KV_MANY8 };  // few rows: 16, 32 to a tile; many rows: four waves, eight
 struct Plan {
   int form, m;      // the kernel, and the rows of one of its tiles
   long units;       // bound on the tiles of rows
@@ -780,25 +788,33 @@ struct Plan {
 Plan plan_of(int T, int B, bool packed, int H, int Hkv, int hd, int max_new, int max_len, int window, int sinks) {
   Plan p;
   const int G = H / Hkv;
-  const long rows = (long)(packed ? (max_new > 0 && max_new < T ? max_new : T) : 1) * G;
-  // 256 rows share a tile's conversion where that still fills the CUs, 128 rows leave less idle where not (us, 256 / 128
-  // rows: 4096 tokens over 32768, 2 heads to a kv head of 128, 985 / 1116; ragged prompts up to 777, 60 / 24; 6000 tokens
-  // under a window of 1024, 4 heads of 64, 76 / 59)
-  const bool wide = hd == 128 && !window && (long)T * G / 256 * Hkv >= uwc_cu_count();
-  p.form = rows <= 32 ? KV_FEW : wide ? KV_MANY8 : KV_MANY4;
-  p.m = p.form == KV_FEW ? 16 : p.form == KV_MANY4 ? 128 : 256;
+  const long cus = uwc_cu_count(), rows = (long)(packed ? (max_new > 0 && max_new < T ? max_new : T) : 1) * G;
+  long keys = max_len > 0 ? max_len : 1;
+  if (window && (long)window + sinks + rows / G + 64 < keys) keys = (long)window + sinks + rows / G + 64;
+  const long tiles = (keys + 63) / 64;
+  // Tiles of 16 rows while at most 80 of them per CU meet a tile of 64 keys (40 of more than 128 rows): they spread best,
+  // and the caches serve a key's second reader. Beyond that up to 32 rows still go so (us, 16 rows / many: 5 tokens of 64 heads to 8
+  // kv heads, 8 sequences of 20000 136 / 113, 1 of 50000 43 / 45; 16 of 32 heads over 3000, 4 sequences 22 / 29, over
+  // 8000, 16 sequences 122 / 98), two tiles of 16 to a wave for heads of 64 and fewer, whose keys cost less to read
+  // than to convert (300 tokens of 16 heads, 600 rows, 10 / 16, 1000 of them 50 / 33; 5 tokens of 7 heads to a kv head of 64, 8 x 20000: 92 -> 67, many 74; heads of 128: 78.6 / 78.2).
+  const bool light = (rows + 15) / 16 * B * Hkv * tiles <= (rows <= 128 ? 80 : 40) * cus;
+  // Many: 256 rows share a tile's conversion where that still fills the CUs, 128 rows leave less idle where not (us, 256 /
+  // 128 rows: 4096 tokens over 32768, 2 heads to a kv head of 128, 985 / 1116; ragged prompts up to 777, 60 / 24; 6000
+  // tokens under a window of 1024, 4 heads of 64, 76 / 59).
+  const bool wide = hd == 128 && !window && (long)T * G / 256 * Hkv >= cus;
+  p.form = light || rows <= 16 ? KV_FEW1 : hd <= 64 && rows <= 48 ? KV_FEW2 : rows <= 32 ? KV_FEW1 : wide ? KV_MANY8 : KV_MANY4;
+  p.m = p.form == KV_FEW1 ? 16 : p.form == KV_FEW2 ? 32 : p.form == KV_MANY4 ? 128 : 256;
   const int M = p.m;
   p.units = packed ? ((long)T * G + M - 1) / M + B : (long)B * ((G + M - 1) / M);
-  long keys = max_len > 0 ? max_len : 1;
-  if (window && (long)window + sinks + M / G + 128 < keys) keys = (long)window + sinks + M / G + 128;
-  const long tiles = (keys + 63) / 64;
-  // Few rows: two workgroups fit a CU. Where sequences and heads alone fill the CUs, their lengths may differ and the
-  // keys are cut into pieces that make four rounds' worth (48 sequences of 1500 to 12000 tokens, 8 kv heads: 153 us;
+  // Two workgroups fit a CU. Where rows and heads alone fill the CUs with few-row tiles, their lengths may differ and the
+  // keys are cut into pieces that make four rounds' worth (48 sequences of 1500 to 12000 tokens, 8 kv heads: 146 us;
   // two per CU 204, none cut 166); where they do not, into as many as fit at once (one of 131072: 55 us with one or two
   // per CU, 59 with four, 68 with eight), down to one tile a wave (one of 2500: 9.7 us; two tiles 11.8, four 15.6).
-  const long wgs = p.units * Hkv, cus = uwc_cu_count();
-  long splits = p.form == KV_FEW ? wgs >= cus ? (4 * cus + wgs - 1) / wgs : 2 * cus / wgs : 2 * cus / wgs;
-  if (splits > (tiles + 3) / 4) splits = (tiles + 3) / 4;
+  const long likely = (long)B * ((rows + M - 1) / M), wgs = (likely < p.units ? likely : p.units) * Hkv;
+  const bool few = p.form <= KV_FEW2, full = wgs >= cus;
+  long splits = few && full ? (4 * cus + wgs - 1) / wgs : 2 * cus / wgs;
+  const long most = (tiles + (few && !full ? 3 : 7)) / (few && !full ? 4 : 8);
+  if (splits > most) splits = most;
   if (splits < 1) splits = 1;
   p.tps = (int)((tiles + splits - 1) / splits);
   p.splits = (int)((tiles + p.tps - 1) / p.tps);
@@ -854,8 +870,9 @@ extern "C" int uwc_kv_attend(const int8_t* k, const int8_t* v, const float* ks, 
 #define KV_MANY(HD, NW) KV_GO((kv_attend_many_kernel<HD, NW, __bf16>), (kv_attend_many_kernel<HD, NW, _Float16>), 64 * NW)
 #define KV_FORMS(HD)                                                                                          \
   do {                                                                                                        \
-    if (p.form == KV_FEW) KV_GO((kv_attend_few_kernel<HD, 1, __bf16>), (kv_attend_few_kernel<HD, 1, _Float16>), 256); \
-    else if (p.form == KV_MANY4) KV_MANY(HD, 4);                                                            \
+    if (p.form == KV_FEW1) KV_GO((kv_attend_few_kernel<HD, 1, __bf16>), (kv_attend_few_kernel<HD, 1, _Float16>), 256); \
+    else if (HD <= 64 && p.form == KV_FEW2) KV_GO((kv_attend_few_kernel<(HD <= 64 ? HD : 64), 2, __bf16>), (kv_attend_few_kernel<(HD <= 64 ? HD : 64), 2, _Float16>), 256); \
+    else if (p.form == KV_MANY4) KV_MANY(HD, 4);                                                              \
     else KV_MANY(HD, 8);                                                                                      \
   } while (0)
   if (hd == 32) KV_FORMS(32);
@@ -863,10 +880,17 @@ extern "C" int uwc_kv_attend(const int8_t* k, const int8_t* v, const float* ks, 
   else KV_FORMS(128);
   if (int st = uwc_launch_status(fn)) return st;
   if (p.splits == 1) return UWC_OK;
-#define KV_JOIN(HD)                                                                                                       \
-  return uwc_launch_rows(fn, T * H, 256, [&](long r0, int n) {                                                            \
-    if (dtype == UWC_KV_BF16) hipLaunchKernelGGL((kv_attend_join_kernel<HD, __bf16>), dim3((unsigned)n), wg, 0, stream, a, r0); \
-    else hipLaunchKernelGGL((kv_attend_join_kernel<HD, _Float16>), dim3((unsigned)n), wg, 0, stream, a, r0);              \
+  const long R = (long)T * H;
+  const bool many = p.splits > 8;
+  const long per = many ? 1 : 1024 / hd;  // rows of a workgroup
+#define KV_JOIN(HD)                                                                                                \
+  return uwc_launch_rows(fn, (int)((R + per - 1) / per), 256, [&](long g0, int n) {                                \
+    const dim3 jg((unsigned)n);                                                                                    \
+    const bool bf = dtype == UWC_KV_BF16;                                                                          \
+    if (many && bf) hipLaunchKernelGGL((kv_attend_join_kernel<HD, true, __bf16>), jg, wg, 0, stream, a, g0, R);    \
+    else if (many) hipLaunchKernelGGL((kv_attend_join_kernel<HD, true, _Float16>), jg, wg, 0, stream, a, g0, R);   \
+    else if (bf) hipLaunchKernelGGL((kv_attend_join_kernel<HD, false, __bf16>), jg, wg, 0, stream, a, g0 * per, R); \
+    else hipLaunchKernelGGL((kv_attend_join_kernel<HD, false, _Float16>), jg, wg, 0, stream, a, g0 * per, R);      \
   })
   if (hd == 32) KV_JOIN(32);
   if (hd == 64) KV_JOIN(64);
