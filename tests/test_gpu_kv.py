@@ -184,6 +184,59 @@ def test_attend_strides_and_scale(dev, new):
         check(kv.attend(cache, q, table.t().contiguous().t(), L, **args), want, tol)
 
 
+HEAVY = [s for s in SHAPES if max(s[0]) * s[2] // s[3] > 16]
+
+
+@pytest.mark.parametrize("new,lens,H,Hkv,hd,page,dtype", HEAVY)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (33, 4), (1000, 70)])
+def test_attend_forms_for_much_work(dev, new, lens, H, Hkv, hd, page, dtype, window, sinks):
+    """The kernels that calls with much work take (a bound of the lengths that is far off takes them here): two row
+    tiles to a wave for heads of 64 and less, 128 rows to a workgroup; with and without splits of the keys."""
+    from uwc_amd import kv
+    cache, q, table, L, cu = problem(dev, new, lens, H, Hkv, hd, page, dtype, seed=len(new) + H)
+    want, tol = R.attend(cache, q, table, L, cu, window, sinks)
+    for bound in (1 << 16, 1 << 22):
+        check(kv.attend(cache, q, table, L, cu=cu, max_new=max(new), max_len=bound, window=window, sinks=sinks), want, tol)
+
+
+@pytest.mark.parametrize("new,lens,dtype", [([2070, 2100], [2100, 2100], BF), ([4200], [5000], HF), ([1500, 1400, 1301], [1500, 1463, 2000], BF)])
+def test_attend_eight_waves(dev, new, lens, dtype):
+    """Enough rows for 256 to a workgroup on every CU, the last tiles of a sequence partly filled."""
+    from uwc_amd import kv
+    cache, q, table, L, cu = problem(dev, new, lens, 16, 16, 128, 32, dtype, seed=len(new))
+    want, tol = R.attend(cache, q, table, L, cu)
+    check(kv.attend(cache, q, table, L, cu=cu, max_new=max(new), max_len=max(lens)), want, tol)
+
+
+def test_short_and_long_way_agree(dev, monkeypatch):
+    """The native way for arguments of the usual form and the one that looks at any: the same bits."""
+    from uwc_amd import _lib, kv
+    cache, qkv, table, c, cos, sin, cu, w = append_problem(dev, [70, 3], [5, 40], 4, 2, 64, 16, HF, True)
+    other = [x.clone() for x in cache]
+
+    def run(cache):
+        q = kv.append(cache, qkv, table, c, cos, sin, cu=cu, q_norm=w[0], k_norm=w[1])
+        n = c + (cu[1:] - cu[:-1])
+        return (q, kv.attend(cache, q, table, n, cu=cu, window=20, sinks=2), kv.attend(cache, q, table, n, cu=cu, max_new=70, scale=0.2),
+                *kv.read(cache, table, c, cu, 73, dtype=HF), *cache)
+
+    short = run(cache)
+
+    class Never:
+        append = attend = read = staticmethod(lambda *a: None)
+
+    monkeypatch.setattr(_lib, "_KV", Never)
+    for a, b in zip(short, run(other)):
+        assert torch.equal(a, b)
+
+
+def test_refusals_of_the_library_reach_the_caller(dev):
+    from uwc_amd import _lib, kv
+    cache, q, table, L, cu = problem(dev, [1], [20], 4, 2, 64, 16, BF)
+    with pytest.raises(_lib.UwcError, match="scale of the scores must be positive"):
+        kv.attend(cache, q, table, L, scale=0.0)
+
+
 def test_offsets_past_32_bits(dev):
     """Pages beyond 2^31 bytes of keys: appended to, attended over, read back."""
     from uwc_amd import kv

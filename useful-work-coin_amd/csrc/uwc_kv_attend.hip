@@ -873,7 +873,7 @@ extern "C" int uwc_kv_attend(const int8_t* k, const int8_t* v, const float* ks, 
     if (p.form == KV_FEW1) KV_GO((kv_attend_few_kernel<HD, 1, __bf16>), (kv_attend_few_kernel<HD, 1, _Float16>), 256); \
     else if (HD <= 64 && p.form == KV_FEW2) KV_GO((kv_attend_few_kernel<(HD <= 64 ? HD : 64), 2, __bf16>), (kv_attend_few_kernel<(HD <= 64 ? HD : 64), 2, _Float16>), 256); \
     else if (p.form == KV_MANY4) KV_MANY(HD, 4);                                                              \
-    else KV_MANY(HD, 8);                                                                                      \
+    else KV_MANY(128, 8); /* heads of 128 alone take it */                                                    \
   } while (0)
   if (hd == 32) KV_FORMS(32);
   else if (hd == 64) KV_FORMS(64);

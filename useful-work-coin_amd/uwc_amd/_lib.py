@@ -126,5 +126,33 @@ def call(name: str, *args) -> None:
     """Call an int-status entry point; raise UwcError with uwc_last_error() on failure."""
     st = getattr(lib(), name)(*args)
     if st != 0:
-        msg = lib().uwc_last_error().decode(errors="replace")
-        raise UwcError(f"{name} failed (status {st}): {msg}")
+        fail(name, st)
+
+
+def fail(name: str, st: int) -> None:
+    """Raise UwcError with uwc_last_error() for a call that returned st."""
+    msg = lib().uwc_last_error().decode(errors="replace")
+    raise UwcError(f"{name} failed (status {st}): {msg}")
+
+
+_KV = None
+
+
+def kv():
+    """_kv.so (uwc_kv_bind.cpp), the short way to the key/value cache's entry points, bound to the
+    library; it has to be built from the same header."""
+    global _KV
+    if _KV is None:
+        L = lib()
+        try:
+            from . import _kv
+        except ImportError as e:
+            raise ImportError(f"{os.path.join(_HERE, '_kv.so')} is not built or does not fit this torch: run "
+                              "useful-work-coin_amd/csrc/build.sh (or __graft_entry__.build())") from e
+        if _kv.header_sha() != L.uwc_header_sha().decode():
+            raise ImportError("_kv.so and libuwc_hip.so were built from different include/uwc.h: rebuild with "
+                              "useful-work-coin_amd/csrc/build.sh (or __graft_entry__.build())")
+        _kv.bind(*(ctypes.cast(f, vp).value for f in (L.uwc_kv_append, L.uwc_kv_attend_scratch_bytes, L.uwc_kv_attend,
+                                                      L.uwc_kv_read)))
+        _KV = _kv
+    return _KV

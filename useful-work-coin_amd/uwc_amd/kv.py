@@ -23,7 +23,9 @@ bfloat16 or float16. Index tensors are int32 on the cache's GPU; nothing here re
 every call can be captured into a graph. A page that a row needs but that is not in the cache (an entry
 outside [0, pages), a position past the table's width) makes that row NaN; nothing else is touched.
 
-Everything runs on torch's current HIP stream; buffers are torch tensors on the caller's GPU.
+Everything runs on torch's current HIP stream; buffers are torch tensors on the caller's GPU. Arguments
+of the usual form (dense, aligned) take a short way through native code; what follows it in each function
+looks at every other form, copies what has to be dense, and refuses.
 """
 from __future__ import annotations
 
@@ -38,6 +40,10 @@ PAGES = (16, 32, 64, 128)
 HEAD_DIMS = (32, 64, 128)
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
 _I32MAX = 2 ** 31 - 1
+
+
+def _stream() -> int:
+    return _lib.stream() if torch.cuda.is_initialized() else 0
 
 
 def _require(ok, msg):
@@ -107,6 +113,9 @@ def append(cache, qkv: torch.Tensor, table: torch.Tensor, ctx: torch.Tensor, cos
     positions x hd) of their positions: x cos + (-hi, lo)(x) sin. A page's scale is max|x| / 127 over the
     tokens it holds; where new ones raise it, the older ones are rounded again. No two sequences' new
     tokens may share a page."""
+    r = _lib.kv().append(*cache, qkv, table, ctx, cos, sin, cu, q_norm, k_norm, eps, _stream())
+    if r is not None:
+        return r if type(r) is not int else _lib.fail("uwc_kv_append", r)
     fn = "kv.append"
     k, v, ks, vs, pages, page, Hkv, hd = _cache(fn, cache)
     dev = cache[0].device
@@ -144,6 +153,9 @@ def attend(cache, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, cu=N
     position p sees keys above p - window, and the sequence's first `sinks`. Rows that see nothing are zeros.
     max_new, max_len: bounds of the sequences' new tokens and lengths that the caller knows, for splitting
     the work well; results are right for any. scale defaults to 1 / sqrt(hd)."""
+    r = _lib.kv().attend(*cache, q, table, lens, cu, max_new, max_len, window, sinks, scale, _stream())
+    if r is not None:
+        return r if type(r) is not int else _lib.fail("uwc_kv_attend", r)
     fn = "kv.attend"
     k, v, ks, vs, pages, page, Hkv, hd = _cache(fn, cache)
     dev = cache[0].device
@@ -178,6 +190,10 @@ def read(cache, table: torch.Tensor, start: torch.Tensor, cu: torch.Tensor, rows
     """Cached tokens as values: keys and values (rows, Hkv, hd) of `dtype`, sequence b's tokens
     start[b] .. start[b] + cu[b + 1] - cu[b] - 1 at rows cu[b] .. cu[b + 1] - 1. rows is cu[B]; rows past it
     are not written."""
+    if dtype in _TYPES:
+        r = _lib.kv().read(*cache, table, start, cu, rows, _TYPES[dtype], _stream())
+        if r is not None:
+            return r if type(r) is not int else _lib.fail("uwc_kv_read", r)
     fn = "kv.read"
     k, v, ks, vs, pages, page, Hkv, hd = _cache(fn, cache)
     dev = cache[0].device
