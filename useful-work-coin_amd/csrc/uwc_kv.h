@@ -44,28 +44,31 @@ __device__ __forceinline__ int kv_new(const KvRows& R, int b) {
 }
 
 // Finds unit number `unit` of the list in which sequence b has count(b) units: its sequence and its index
-// there, the same in every lane of the wave. False past the list's end; unit then holds its distance from it.
+// there, uniform over the wave as `unit` has to be. False past the list's end; unit then holds its distance from it.
 template <class F>
 __device__ __forceinline__ bool kv_find(int& unit, int B, F&& count, int& b, int& j) {
   const int lane = threadIdx.x & 63;
+  int n = lane < B ? count(lane) : 0;
   for (int base = 0; base < B; base += 64) {
-    const int n = base + lane < B ? count(base + lane) : 0;
+    const int next = base + 64 + lane < B ? count(base + 64 + lane) : 0;
+    // the inclusive sums over the lanes: within rows of 16, then of the rows before
     int s = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int up = __shfl_up(s, d, 64);
-      if (lane >= d) s += up;
-    }
-    const int total = __shfl(s, 63, 64);
+    s += __builtin_amdgcn_update_dpp(0, s, 0x111, 0xf, 0xf, true);  // row_shr:1, :2, :4, :8
+    s += __builtin_amdgcn_update_dpp(0, s, 0x112, 0xf, 0xf, true);
+    s += __builtin_amdgcn_update_dpp(0, s, 0x114, 0xf, 0xf, true);
+    s += __builtin_amdgcn_update_dpp(0, s, 0x118, 0xf, 0xf, true);
+    s += __builtin_amdgcn_update_dpp(0, s, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+    s += __builtin_amdgcn_update_dpp(0, s, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+    const int total = __builtin_amdgcn_readlane(s, 63);
     if (unit < total) {
       const int l = __builtin_ctzll(__ballot(s > unit));
-      b = __builtin_amdgcn_readfirstlane(base + l);
-      j = __builtin_amdgcn_readfirstlane(unit - (__shfl(s, l, 64) - __shfl(n, l, 64)));
+      b = base + l;
+      j = unit - (__builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(n, l));
       return true;
     }
     unit -= total;
+    n = next;
   }
-  unit = __builtin_amdgcn_readfirstlane(unit);
   return false;
 }
 

@@ -94,8 +94,16 @@ __device__ __forceinline__ bool any_seen(const AttendArgs& a, const Span& s, int
 __device__ __forceinline__ bool all_seen(const AttendArgs& a, const Span& s, int key0, int count) {
   return key0 + count - 1 <= s.p_lo && (!a.window || key0 > s.p_hi - a.window || key0 + count <= a.sinks);
 }
-__device__ __forceinline__ bool seen(const AttendArgs& a, int pos, int key) {
-  return key <= pos && (!a.window || key > pos - a.window || key < a.sinks);
+// Bit j: does a query at pos see key key0 + j?
+__device__ __forceinline__ u32 seen32(const AttendArgs& a, int pos, int key0) {
+  auto below = [](int n) KV_AI { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
+  const u32 m = below(pos - key0 + 1);
+  return a.window ? m & (~below(pos - a.window + 1 - key0) | below(a.sinks - key0)) : m;
+}
+// v where bit j of m is set, else -inf
+__device__ __forceinline__ float pick(u32 m, int j, float v) {
+  const u32 t = (u32)__builtin_amdgcn_sbfe((int)m, j, 1);
+  return __uint_as_float((t & __float_as_uint(v)) | (~t & 0xff800000u));
 }
 
 // The page of the granule that starts at key0: 0 where no row needs it, -1 where one does and there is none.
@@ -326,9 +334,9 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(AttendArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; i++) e[i] = __builtin_fmaf(s[rb][i >> 2][i & 3], Ak, lv);
       if (!whole) {
-        asm volatile("" : "+v"(pos[rb]));  // keeps this a branch
+        const u32 m = seen32(a, pos[rb], kt * 64 + 16 * g);
 #pragma unroll
-        for (int i = 0; i < 16; i++) e[i] = seen(a, pos[rb], kt * 64 + 16 * g + i) ? e[i] : -__builtin_inff();
+        for (int i = 0; i < 16; i++) e[i] = pick(m, i, e[i]);
       }
 #pragma unroll
       for (int i = 0; i < 16; i++) top = fmaxf(top, e[i]);
@@ -428,7 +436,7 @@ __device__ __forceinline__ int v_piece(int r, int c) { return r * 8 + (c ^ ((r ^
 // The weights of one 32-row block for a tile of 64 keys: p the operands of V's products, m the running maximum and
 // l this lane's part of the denominator brought up to date, o rescaled where m moved.
 template <int DB>
-__device__ __forceinline__ void softmax_tile(const AttendArgs& a, f16v s[2], float A, int& pos, bool whole, int key0,
+__device__ __forceinline__ void softmax_tile(const AttendArgs& a, f16v s[2], float A, int pos, bool whole, int key0,
                                              const float4* meta, f16v* o, float& mr, float& l, h8v p[4]) {
   // 2^(s Ak + lk - m) is the weight; Ak > 0, so the maximum of s gives that of the exponent
   float Ak[4], lk[4], rv[4], top = -__builtin_inff();
@@ -438,16 +446,12 @@ __device__ __forceinline__ void softmax_tile(const AttendArgs& a, f16v s[2], flo
     Ak[n] = A * mt.x, lk[n] = mt.y, rv[n] = mt.z;
   }
   if (!whole) {
-    asm volatile("" : "+v"(pos));  // keeps this a branch
+    const u32 seen[2] = {seen32(a, pos, key0), seen32(a, pos, key0 + 32)};
 #pragma unroll
     for (int n = 0; n < 4; n++) {
-      bool some = false;
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const bool y = seen(a, pos, key0 + 16 * n + i);
-        s[n >> 1][8 * (n & 1) + i] = y ? s[n >> 1][8 * (n & 1) + i] : -__builtin_inff();
-        some |= y;
-      }
+      for (int i = 0; i < 8; i++) s[n >> 1][8 * (n & 1) + i] = pick(seen[n >> 1], 16 * (n & 1) + i, s[n >> 1][8 * (n & 1) + i]);
+      const bool some = seen[n >> 1] & 0xffu << 16 * (n & 1);
       // -inf has to stay -inf, also under a scale of 0, and under any scale of keys this row does not see
       Ak[n] = !some ? 1.0f : Ak[n] == 0.0f ? 0x1p-126f : Ak[n];
       lk[n] = some ? lk[n] : 0.0f;
@@ -490,7 +494,7 @@ __device__ __forceinline__ void lds_put(u32 a, h8v v) { *(lds_h8)(uintptr_t)a = 
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <int HD, int NW, class T>
-__global__ __launch_bounds__(64 * NW, 2) void kv_attend_many_kernel(AttendArgs a) {
+__global__ __launch_bounds__(64 * NW, HD <= 64 ? 3 : 2) void kv_attend_many_kernel(AttendArgs a) {
   typedef typename kv_vec<T>::v8 v8;
   constexpr bool TURNS = NW == 8;
   constexpr int M = 32 * NW, NT = 64 * NW, KS = HD / 16, DB = HD / 32, STAGES = TURNS ? 4 : 2;
@@ -509,11 +513,14 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attend_many_kernel(AttendArgs a
 
   const int r = x.r0 + wave * 32 + m32;
   const Place mine = place_of(a, x, r, h);
-  int pos = mine.t < 0 ? -1 : x.pos(a, r);
+  const int pos = mine.t < 0 ? -1 : x.pos(a, r);
   const T* qp = static_cast<const T*>(a.q) + (mine.t < 0 ? 0 : mine.t * a.q_stride + mine.head * HD);
 
   const int last_r = x.r0 + M < x.rows ? x.r0 + M - 1 : x.rows - 1;
   const Span sp = span_of(a, x.pos(a, x.r0), x.pos(a, last_r));
+  Span of_wave = sp;  // what the wave's own rows see
+  of_wave.p_lo = uniform(x.pos(a, min(x.r0 + wave * 32, last_r)));
+  of_wave.p_hi = uniform(x.pos(a, min(x.r0 + wave * 32 + 31, last_r)));
   const int t0 = split * a.tps, n = uniform((split + 1 == a.splits ? sp.n : min(sp.n, (split + 1) * a.tps)) - t0);
 
   // The pages and scales of 16 tiles at a time, by the first wave, a lane a granule: the table is read at a step
@@ -596,7 +603,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attend_many_kernel(AttendArgs a
       return sv[stage * ROOM + 32 * db * 8 + v_piece(m32, 2 * g + hf)];
     };
     // products 0 .. 4 DB - 1 are those of a tile's weights with its values, the rest the next tile's scores
-    constexpr int NV = 4 * DB, NP = NV + 2 * KS, PRE = 6;
+    constexpr int NV = 4 * DB, NP = NV + 2 * KS, PRE = HD == 64 ? 4 : 6;
     auto frag = [&](int S, int k) KV_AI {
       return k < NV ? v_frag(S % STAGES, k % DB, k / DB) : k_frag((S + 1) % STAGES, (k - NV) & 1, (k - NV) >> 1);
     };
@@ -675,7 +682,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv_attend_many_kernel(AttendArgs a
             load_piece(i + 2, k);
           }
       const int key0 = sp.tile(t0 + i) * 64;
-      softmax_tile<DB>(a, s, A, pos, all_seen(a, sp, key0, 64), key0 + 8 * hf, meta[i & 31], o, mr, l, p);
+      softmax_tile<DB>(a, s, A, pos, all_seen(a, of_wave, key0, 64), key0 + 8 * hf, meta[i & 31], o, mr, l, p);
       __builtin_amdgcn_sched_barrier(0);
       lds_barrier();
       __builtin_amdgcn_sched_barrier(0);
