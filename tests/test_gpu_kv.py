@@ -148,6 +148,22 @@ def test_attend_value_scales_far_apart(dev, new):
     assert kv.attend(cache, q, table, L, cu=cu, max_new=new).abs().max().item() == 0.0
 
 
+@pytest.mark.parametrize("new", [1, 100])
+def test_attend_scores_far_below_zero(dev, new):
+    """All scores of a row near -1e33: the softmax is that of their differences (here: of one key each)."""
+    from uwc_amd import kv
+    cache, q, table, L, cu = problem(dev, [new], [130], 2, 1, 64, 16, BF)
+    cache[0].copy_(cache[0].abs().clamp(min=1))
+    q = -q.abs().clamp(min=0.5)
+    cache[2].fill_(1e31)
+    want, _ = R.attend(cache, q, table, L, cu)
+    v = R.tokens(cache, table[0], 130)[1][:, 0]
+    got = kv.attend(cache, q, table, L, cu=cu, max_new=new).double()
+    # scores' fp32 roundings pick among keys whose scores are nearly the same: the output is some key's values
+    near = (got[:, :, None] - v[None, None]).abs().amax(-1).amin(-1)
+    assert (near <= 2.0 ** -8 * v.abs().max()).all() and (got - want).abs().amax(-1).le(2.0 ** -8 * v.abs().max()).float().mean() > 0.9
+
+
 @pytest.mark.parametrize("new", [1, 64])
 def test_attend_queries_that_are_not_numbers(dev, new):
     """An infinite or NaN query gives NaN in its own row and head, and nowhere else."""

@@ -48,7 +48,7 @@ struct AttendArgs {
   float2* ml;  // splits x T H: their m and denominator
 };
 
-constexpr float KV_LOWEST = -1e30f;  // m of a row that has seen nothing
+constexpr float KV_LOWEST = -3e38f;  // m of a row that has seen nothing: differences from it stay numbers
 constexpr float KV_SLACK = 8.0f;
 
 // bytes of w as four fp16: 0x6400 | (x + 128) is 1024 + x + 128 in fp16, and subtracting 1152 is exact
