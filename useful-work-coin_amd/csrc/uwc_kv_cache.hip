@@ -263,18 +263,27 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int unit, int h
   }
 }
 
-// Workgroups: first `units` x 2 Hkv for the pages, then one for every four rows of q.
+// Workgroups: first `units` x 2 Hkv for the pages, then one for every four rows of q. Consecutive workgroups go to
+// consecutive XCDs, so they are dealt such that all heads of a page, and 64 consecutive rows of q, share an XCD and
+// with it the rotation's rows in its L2 (a prefill of 3890 tokens in three sequences, 16 + 2 x 8 heads of 128:
+// 17.3 us heads over the XCDs, 15.8 so; eights of pages and of rows in turn 18.1).
 template <int HD, int ROUNDS, class T>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
-  const u32 pages = (u32)a.units * 2u * (u32)a.Hkv;
+  const u32 sides = 2u * (u32)a.Hkv, pages = (u32)a.units * sides;
   if (blockIdx.x >= pages) {
-    const int row = __builtin_amdgcn_readfirstlane((int)((blockIdx.x - pages) * 4 + (threadIdx.x >> 6)));
+    u32 i = blockIdx.x - pages;
+    if (i < (gridDim.x - pages) / 128 * 128) i = i / 128 * 128 + i % 8 * 16 + i % 128 / 8;
+    const int row = __builtin_amdgcn_readfirstlane((int)(i * 4 + (threadIdx.x >> 6)));
     if (row < a.rows.T) append_q<HD, T>(a, row);
     return;
   }
-  const int unit = blockIdx.x / (2 * a.Hkv), sh = blockIdx.x % (2 * a.Hkv);
-  if (sh < a.Hkv) append_page<HD, ROUNDS, 0, T>(a, unit, sh);
-  else append_page<HD, ROUNDS, 1, T>(a, unit, sh - a.Hkv);
+  u32 unit = blockIdx.x / sides, sh = blockIdx.x % sides;
+  if (unit < ((u32)a.units & ~7u)) {
+    const u32 r = blockIdx.x % (8 * sides);
+    unit = blockIdx.x / (8 * sides) * 8 + r % 8, sh = r / 8;
+  }
+  if (sh < (u32)a.Hkv) append_page<HD, ROUNDS, 0, T>(a, (int)unit, (int)sh);
+  else append_page<HD, ROUNDS, 1, T>(a, (int)unit, (int)sh - a.Hkv);
 }
 
 // past the caches: values that are written once (a prefix of 30000 tokens, 184 MB moved: 42.3 -> 36.0 us)
