@@ -42,7 +42,7 @@ struct AttendArgs {
   int H, Hkv, G, lp;
   int window, sinks;
   float c;  // scale * log2(e)
-  int units, splits, tps;
+  int units, splits, tps, fold;
   void* o;
   float* po;   // splits x T H x hd: unnormalised outputs, when splits > 1
   float2* ml;  // splits x T H: their m and denominator
@@ -504,7 +504,10 @@ __global__ __launch_bounds__(64 * NW, HD <= 64 ? 3 : 2) void kv_attend_many_kern
   __shared__ int ids[32][4];      // their pages
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), hf = lane >> 5, m32 = lane & 31;
   const int h = blockIdx.x % a.Hkv, rest = blockIdx.x / a.Hkv, split = rest % a.splits;
-  int u = a.units - 1 - rest / a.splits;  // the last rows of a sequence see the most keys: first
+  // The last rows of a sequence see the most keys: first. Where all workgroups fit at once (fold), the second half goes
+  // from the fewest keys up, so that a CU's two make up for each other.
+  const int nth = rest / a.splits, half = a.units >> 1;
+  int u = a.fold && nth >= half ? nth - half : a.units - 1 - nth;
   Unit x;
   if (!unit_of(a, u, M, x)) {
     zero_rows<HD, T>(a, u, M, h, split);
@@ -866,7 +869,7 @@ extern "C" int uwc_kv_attend(const int8_t* k, const int8_t* v, const float* ks, 
   const long blocks = p.units * p.splits * Hkv;
   if (blocks > 0xFFFFFF) return uwc_fail("%s: too many tokens (%d) and heads (%d)", fn, T, H);  // 2^32 threads
   AttendArgs a{k, v, ks, vs, pages, q, q_stride, table, table_stride, width, lens, {cu, B, T}, H, Hkv, H / Hkv,
-               __builtin_ctz((unsigned)page), window, sinks, scale * 1.4426950408889634f, (int)p.units, p.splits, p.tps, o,
+               __builtin_ctz((unsigned)page), window, sinks, scale * 1.4426950408889634f, (int)p.units, p.splits, p.tps, blocks <= 2L * uwc_cu_count(), o,
                static_cast<float*>(scratch), reinterpret_cast<float2*>(static_cast<char*>(scratch) + p.o_bytes)};
   const dim3 grid((unsigned)blocks), wg(256);
 #define KV_GO(KERNEL_BF16, KERNEL_FP16, threads)                                                                  \
