@@ -821,16 +821,57 @@ Plan plan_of(int T, int B, bool packed, int H, int Hkv, int hd, int max_new, int
   // two per CU 204, none cut 166); where they do not, into as many as fit at once (one of 131072: 55 us with one or two
   // per CU, 59 with four, 68 with eight), down to one tile a wave (one of 2500: 9.7 us; two tiles 11.8, four 15.6).
   const long likely = (long)B * ((rows + M - 1) / M), wgs = (likely < p.units ? likely : p.units) * Hkv;
-  const bool few = p.form <= KV_FEW2, full = wgs >= cus;
-  long splits = few && full ? (4 * cus + wgs - 1) / wgs : 2 * cus / wgs;
-  const long most = (tiles + (few && !full ? 3 : 7)) / (few && !full ? 4 : 8);
-  if (splits > most) splits = most;
-  if (splits < 1) splits = 1;
+  // Many rows: what a split saves in steps of about 1.5 us against what the join costs, a launch and its parts' bytes
+  // (1000 tokens of 16 heads over 4000: 66 us in four, 75 in two, 118 in one; 2 x 1000 over none, heads of 64, 22 in one,
+  // 30 in two).
+  long splits = 1;
+  if (p.form <= KV_FEW2) {
+    const bool full = wgs >= cus;
+    splits = full ? (4 * cus + wgs - 1) / wgs : 2 * cus / wgs;
+    const long most = (tiles + (full ? 7 : 3)) / (full ? 8 : 4);
+    if (splits > most) splits = most;
+    if (splits < 1) splits = 1;
+  } else {
+    double best = 1e30;
+    for (long s = 1; s == 1 || (s <= 2 * cus / wgs && s <= (tiles + 7) / 8); s++) {
+      const double us = 1.5 * ((tiles + s - 1) / s) + (s > 1 ? 7.0 + (double)s * T * H * hd * 8 / 4.8e6 : 0.0);
+      if (us < best) best = us, splits = s;
+      else if (s > 2 * splits + 8) break;  // past the least
+    }
+  }
   p.tps = (int)((tiles + splits - 1) / splits);
   p.splits = (int)((tiles + p.tps - 1) / p.tps);
   p.o_bytes = p.splits > 1 ? (uint64_t)p.splits * T * H * hd * 4 : 0;
   p.bytes = p.splits > 1 ? p.o_bytes + (uint64_t)p.splits * T * H * 8 : 0;
   return p;
+}
+
+template <int HD, class T>
+bool launch_typed(const Plan& p, const AttendArgs& a, dim3 grid, hipStream_t stream) {
+  if (p.form == KV_FEW1) {
+    hipLaunchKernelGGL((kv_attend_few_kernel<HD, 1, T>), grid, dim3(256), 0, stream, a);
+    return true;
+  }
+  if (p.form == KV_MANY4) {
+    hipLaunchKernelGGL((kv_attend_many_kernel<HD, 4, T>), grid, dim3(256), 0, stream, a);
+    return true;
+  }
+  if constexpr (HD <= 64) {
+    if (p.form == KV_FEW2) {
+      hipLaunchKernelGGL((kv_attend_few_kernel<HD, 2, T>), grid, dim3(256), 0, stream, a);
+      return true;
+    }
+  } else {
+    if (p.form == KV_MANY8) {
+      hipLaunchKernelGGL((kv_attend_many_kernel<HD, 8, T>), grid, dim3(512), 0, stream, a);
+      return true;
+    }
+  }
+  return false;  // the heads have no such form
+}
+template <int HD>
+bool launch(const Plan& p, const AttendArgs& a, int dtype, dim3 grid, hipStream_t stream) {
+  return dtype == UWC_KV_BF16 ? launch_typed<HD, __bf16>(p, a, grid, stream) : launch_typed<HD, _Float16>(p, a, grid, stream);
 }
 
 }  // namespace
@@ -872,22 +913,9 @@ extern "C" int uwc_kv_attend(const int8_t* k, const int8_t* v, const float* ks, 
                __builtin_ctz((unsigned)page), window, sinks, scale * 1.4426950408889634f, (int)p.units, p.splits, p.tps, blocks <= 2L * uwc_cu_count(), o,
                static_cast<float*>(scratch), reinterpret_cast<float2*>(static_cast<char*>(scratch) + p.o_bytes)};
   const dim3 grid((unsigned)blocks), wg(256);
-#define KV_GO(KERNEL_BF16, KERNEL_FP16, threads)                                                                  \
-  do {                                                                                                            \
-    if (dtype == UWC_KV_BF16) hipLaunchKernelGGL((KERNEL_BF16), grid, dim3(threads), 0, stream, a);               \
-    else hipLaunchKernelGGL((KERNEL_FP16), grid, dim3(threads), 0, stream, a);                                    \
-  } while (0)
-#define KV_MANY(HD, NW) KV_GO((kv_attend_many_kernel<HD, NW, __bf16>), (kv_attend_many_kernel<HD, NW, _Float16>), 64 * NW)
-#define KV_FORMS(HD)                                                                                          \
-  do {                                                                                                        \
-    if (p.form == KV_FEW1) KV_GO((kv_attend_few_kernel<HD, 1, __bf16>), (kv_attend_few_kernel<HD, 1, _Float16>), 256); \
-    else if (HD <= 64 && p.form == KV_FEW2) KV_GO((kv_attend_few_kernel<(HD <= 64 ? HD : 64), 2, __bf16>), (kv_attend_few_kernel<(HD <= 64 ? HD : 64), 2, _Float16>), 256); \
-    else if (p.form == KV_MANY4) KV_MANY(HD, 4);                                                              \
-    else KV_MANY(128, 8); /* heads of 128 alone take it */                                                    \
-  } while (0)
-  if (hd == 32) KV_FORMS(32);
-  else if (hd == 64) KV_FORMS(64);
-  else KV_FORMS(128);
+  const bool launched = hd == 32 ? launch<32>(p, a, dtype, grid, stream) : hd == 64 ? launch<64>(p, a, dtype, grid, stream)
+                                                                                    : launch<128>(p, a, dtype, grid, stream);
+  if (!launched) return uwc_fail("%s: no kernel of form %d for heads of %d", fn, p.form, hd);
   if (int st = uwc_launch_status(fn)) return st;
   if (p.splits == 1) return UWC_OK;
   const long R = (long)T * H;
