@@ -417,8 +417,8 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(AttendArgs a) {
 // step i, when values i - 1 are done with. Eight waves keep four stages of either, as the waves that are half a
 // step behind still read values i when the others are a half past them, and write tile i + 2 in step i's second half.
 //
-// LDS rows hold 16-byte pieces (8 fp16), piece c of row r at c ^ swz(r), so that the 32 rows of an operand are
-// read without bank conflicts. K's operand row m is key 16 (m >> 4) + 8 (m >> 2 & 1) + 4 (m >> 3 & 1) +
+// LDS rows hold 16-byte pieces (8 fp16), piece c of row r at c ^ swz(r), such that 16 lanes, which LDS serves at once,
+// hit all of its 64 banks: 16 rows of an operand that are read, two key rows or four value rows that are written. K's operand row m is key 16 (m >> 4) + 8 (m >> 2 & 1) + 4 (m >> 3 & 1) +
 // (m & 3) of its 32: the scores of lane half hf are then keys 16 n + 8 hf + i, the 8 k slots of V's product n.
 //
 // Measured: 4096 tokens over 32768, 16 heads of 128, 985 us = 1048 TFLOP/s at a clock that the load drives down to
@@ -428,8 +428,7 @@ __device__ __forceinline__ int key_row(int key) { return (key & ~12) | ((key & 4
 template <int HD>
 __device__ __forceinline__ int k_piece(int r, int c) {  // of rows of HD fp16
   if (HD == 32) return r * 4 + (c ^ ((r >> 1) & 3));
-  if (HD == 128) c = c >> 1 | (c & 1) << 3;  // the eight lanes that write a row's even pieces hit all banks
-  return r * (HD / 8) + (c ^ ((r ^ (r >> 3 & 3)) & 7));
+  return HD == 128 ? r * 16 + (c ^ (r & 15)) : r * 8 + (c ^ ((r ^ (r >> 3 & 3)) & 7));
 }
 __device__ __forceinline__ int v_piece(int r, int c) { return r * 8 + (c ^ ((r ^ (r >> 3 & 3)) & 7)); }
 
@@ -595,8 +594,8 @@ __global__ __launch_bounds__(64 * NW, HD <= 64 ? 3 : 2) void kv_attend_many_kern
       const int off = (sp.tile(t0 + i) * 64) & mask;  // pages of 64 and fewer start with a tile
       st[k] = *reinterpret_cast<const u4v*>((of_values(k) ? vh + off : kh + off * HD) + ((u64)(u32)max(idp[k], 0) * page_bytes + poff[k]));
     };
-    auto half_to_lds = [&](int i, int k, int half) KV_AI {  // the second half lies 8 pieces on in the keys' rows of 16, else 1
-      const u32 to = half ? dst[k] ^ (HD == 128 && !of_values(k) ? 128 : 16) : dst[k];
+    auto half_to_lds = [&](int i, int k, int half) KV_AI {
+      const u32 to = half ? dst[k] ^ 16 : dst[k];
       lds_put(to + i % STAGES * ROOM * 16, to_half8(st[k][2 * half], st[k][2 * half + 1]));
     };
     auto k_frag = [&](int stage, int kb, int ks) KV_AI {
@@ -816,7 +815,7 @@ Plan plan_of(int T, int B, bool packed, int H, int Hkv, int hd, int max_new, int
   p.m = p.form == KV_FEW1 ? 16 : p.form == KV_FEW2 ? 32 : p.form == KV_MANY4 ? 128 : 256;
   const int M = p.m;
   p.units = packed ? ((long)T * G + M - 1) / M + B : (long)B * ((G + M - 1) / M);
-  // Two workgroups fit a CU. Where rows and heads alone fill the CUs with few-row tiles, their lengths may differ and the
+  // Two workgroups of four waves fit a CU. Where rows and heads alone fill the CUs with few-row tiles, their lengths may differ and the
   // keys are cut into pieces that make four rounds' worth (48 sequences of 1500 to 12000 tokens, 8 kv heads: 146 us;
   // two per CU 204, none cut 166); where they do not, into as many as fit at once (one of 131072: 55 us with one or two
   // per CU, 59 with four, 68 with eight), down to one tile a wave (one of 2500: 9.7 us; two tiles 11.8, four 15.6).
@@ -833,7 +832,8 @@ Plan plan_of(int T, int B, bool packed, int H, int Hkv, int hd, int max_new, int
     if (splits < 1) splits = 1;
   } else {
     double best = 1e30;
-    for (long s = 1; s == 1 || (s <= 2 * cus / wgs && s <= (tiles + 7) / 8); s++) {
+    const long fit = (p.form == KV_MANY8 ? 1 : 2) * cus / wgs;  // eight waves fill a CU
+    for (long s = 1; s == 1 || (s <= fit && s <= (tiles + 7) / 8); s++) {
       const double us = 1.5 * ((tiles + s - 1) / s) + (s > 1 ? 7.0 + (double)s * T * H * hd * 8 / 4.8e6 : 0.0);
       if (us < best) best = us, splits = s;
       else if (s > 2 * splits + 8) break;  // past the least
