@@ -426,6 +426,33 @@ def test_read_is_the_rounded_product(dev, dtype, hd, page, Hkv):
     assert not torch.isnan(ko[66 + first:]).any() and not torch.isnan(vo[66 + first:]).any()
 
 
+def test_no_sequences(dev):
+    """A padded batch without a sequence: zeros."""
+    from uwc_amd import kv
+    cache = kv.new_cache(2, 2, 64, 16, dev)
+    table, none, cu = torch.zeros((0, 3), dtype=torch.int32, device=dev), R.ints([], dev), R.ints([0], dev)
+    q = torch.ones((70, 4, 64), dtype=BF, device=dev)
+    assert not kv.attend(cache, q, table, none, cu=cu).any()
+    cos = torch.ones((4, 64), device=dev)
+    assert not kv.append(cache, torch.ones((9, 8 * 64), dtype=BF, device=dev), table, none, cos, cos, cu=cu).any()
+
+
+@pytest.mark.parametrize("new", [1, 5, 300])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 3), (2 ** 31 - 1, 2 ** 31 - 1)])
+def test_attend_lengths_past_the_table(dev, new, window, sinks):
+    """Lengths that no table could hold end at once, in NaN; another sequence beside is as it was."""
+    from uwc_amd import kv
+    cache, q, table, L, cu = problem(dev, [new, new], [400, 400], 8, 2, 64, 16, BF)
+    want, tol = R.attend(cache, q, table, L, cu, window if window < 1000 else 0, sinks if window < 1000 else 0)
+    L[0] = 2 ** 31 - 100
+    got = kv.attend(cache, q, table, L, cu=cu, max_new=new, max_len=400, window=window, sinks=sinks)
+    assert torch.isnan(got[:new]).all()
+    check(got[new:], want[new:], tol[new:])
+    got = kv.attend(cache, q, table, L, cu=cu, max_new=new, max_len=1 << 22, window=window, sinks=sinks)
+    assert torch.isnan(got[:new]).all()
+    check(got[new:], want[new:], tol[new:])
+
+
 def test_nothing_to_do(dev):
     from uwc_amd import kv
     cache = kv.new_cache(2, 2, 64, 16, dev)

@@ -82,9 +82,11 @@ __device__ __forceinline__ Span span_of(const AttendArgs& a, int p_lo, int p_hi)
   s.p_lo = p_lo = uniform(p_lo), s.p_hi = p_hi = uniform(p_hi);
   s.lo = a.window && p_lo >= a.window ? p_lo - a.window + 1 : 0;
   s.lt = s.lo >> 6;
-  const int first = (a.sinks + 63) >> 6;
-  s.st = first < s.lt ? first : s.lt;
-  s.n = p_hi < 0 ? 0 : s.st + (p_hi >> 6) - s.lt + 1;
+  // Lengths and sinks far past the table's last page (there are no keys: NaN) take no more tiles than it needs to show.
+  const long end = ((long)a.width << a.lp) >> 6, last = (end > s.lt ? end : s.lt) + ((p_hi - p_lo) >> 6) + 1;
+  const int first = (a.sinks + 63) >> 6, head = first < s.lt ? first : s.lt;
+  s.st = head <= end ? head : (int)end + 1;
+  s.n = p_hi < 0 ? 0 : s.st + (int)((p_hi >> 6) < last ? p_hi >> 6 : last) - s.lt + 1;
   return s;
 }
 // Does any row see a key of key0 .. key0 + count - 1? Do all rows see all of them?
@@ -824,7 +826,9 @@ Plan plan_of(int T, int B, bool packed, int H, int Hkv, int hd, int max_new, int
   // keys are cut into pieces that make four rounds' worth (48 sequences of 1500 to 12000 tokens, 8 kv heads: 146 us;
   // two per CU 204, none cut 166); where they do not, into as many as fit at once (one of 131072: 55 us with one or two
   // per CU, 59 with four, 68 with eight), down to one tile a wave (one of 2500: 9.7 us; two tiles 11.8, four 15.6).
-  const long likely = (long)B * ((rows + M - 1) / M), wgs = (likely < p.units ? likely : p.units) * Hkv;
+  long likely = (long)B * ((rows + M - 1) / M);
+  likely = likely < 1 ? 1 : likely < p.units ? likely : p.units;
+  const long wgs = likely * Hkv;
   // Many rows: what a split saves in steps of about 1.5 us against what the join costs, a launch and its parts' bytes
   // (1000 tokens of 16 heads over 4000: 66 us in four, 75 in two, 118 in one; 2 x 1000 over none, heads of 64, 22 in one,
   // 30 in two).
@@ -883,7 +887,8 @@ bool launch(const Plan& p, const AttendArgs& a, int dtype, dim3 grid, hipStream_
 
 extern "C" uint64_t uwc_kv_attend_scratch_bytes(int T, int B, int packed, int H, int Hkv, int hd, int max_new, int max_len,
                                                 int window, int sinks) {
-  if (T <= 0 || B <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || hd <= 0 || window < 0 || sinks < 0) return 0;
+  if (T <= 0 || B < 0 || H <= 0 || Hkv <= 0 || H % Hkv || hd <= 0 || window < 0 || sinks < 0) return 0;
+  window = window < 1 << 30 ? window : 1 << 30, sinks = sinks < 1 << 30 ? sinks : 1 << 30;
   return plan_of(T, B, packed != 0, H, Hkv, hd, max_new, max_len, window, sinks).bytes;
 }
 
@@ -900,10 +905,12 @@ extern "C" int uwc_kv_attend(const int8_t* k, const int8_t* v, const float* ks, 
   if (dtype != UWC_KV_BF16 && dtype != UWC_KV_FP16) return uwc_fail("%s: unknown dtype %d", fn, dtype);
   if (H <= 0 || H % Hkv) return uwc_fail("%s: H=%d is no multiple of Hkv=%d", fn, H, Hkv);
   if (T < 0 || B < 0 || width < 0 || table_stride < 0) return uwc_fail("%s: bad T=%d B=%d width=%d", fn, T, B, width);
+  // positions stay far below 2^30: what is larger is as good as that
+  window = window < 1 << 30 ? window : 1 << 30, sinks = sinks < 1 << 30 ? sinks : 1 << 30;
   if (!(scale > 0.0f) || scale > 3e38f) return uwc_fail("%s: the scale of the scores must be positive", fn);
   if (window < 0 || sinks < 0 || (sinks && !window)) return uwc_fail("%s: bad window=%d sinks=%d", fn, window, sinks);
-  if (T == 0 || B == 0) return UWC_OK;
-  if (!q || !table || !lens || !o) return uwc_fail("%s: null arguments", fn);
+  if (T == 0) return UWC_OK;
+  if (!q || !o || (B && (!table || !lens))) return uwc_fail("%s: null arguments", fn);
   if (!cu && T != B) return uwc_fail("%s: without cu every sequence has one row (T=%d B=%d)", fn, T, B);
   if (q_stride % 8 || (((uintptr_t)q | (uintptr_t)o | (uintptr_t)k | (uintptr_t)v | (uintptr_t)scratch) & 15))
     return uwc_fail("%s: q, o, k, v and scratch must be 16-byte aligned", fn);

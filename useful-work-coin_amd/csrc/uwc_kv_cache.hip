@@ -89,6 +89,7 @@ struct AppendArgs {
   float *ks, *vs;
   void* q;
   int units;  // bound on the pages touched
+  bool deal;  // whole pages to one XCD
 };
 
 __device__ __forceinline__ long page_of(const AppendArgs& a, int b, int col) {
@@ -266,21 +267,23 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int unit, int h
 }
 
 // Workgroups: first `units` x 2 Hkv for the pages, then one for every four rows of q. Consecutive workgroups go to
-// consecutive XCDs, so they are dealt such that all heads of a page, and 64 consecutive rows of q, share an XCD and
-// with it the rotation's rows in its L2 (a prefill of 3890 tokens in three sequences, 16 + 2 x 8 heads of 128:
-// 17.3 us heads over the XCDs, 15.8 so; eights of pages and of rows in turn 18.1).
+// consecutive XCDs. Where sequences have several new tokens (deal), they are dealt such that all heads of a page, and 64
+// consecutive rows of q, share an XCD and with it the rotation's rows in its L2 (a prefill of 3890 tokens in three
+// sequences, 16 + 2 x 8 heads of 128: 17.3 us heads over the XCDs, 15.8 so; eights of pages and of rows in turn 18.1).
+// With a token each a head stays on the XCD whose L2 the kernels that read it next look into (96 sequences, with the
+// read-back 13.7 us, dealt 14.9).
 template <int HD, int ROUNDS, class T>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a) {
   const u32 sides = 2u * (u32)a.Hkv, pages = (u32)a.units * sides;
   if (blockIdx.x >= pages) {
     u32 i = blockIdx.x - pages;
-    if (i < (gridDim.x - pages) / 128 * 128) i = i / 128 * 128 + i % 8 * 16 + i % 128 / 8;
+    if (a.deal && i < (gridDim.x - pages) / 128 * 128) i = i / 128 * 128 + i % 8 * 16 + i % 128 / 8;
     const int row = __builtin_amdgcn_readfirstlane((int)(i * 4 + (threadIdx.x >> 6)));
     if (row < a.rows.T) append_q<HD, T>(a, row);
     return;
   }
   u32 unit = blockIdx.x / sides, sh = blockIdx.x % sides;
-  if (unit < ((u32)a.units & ~7u)) {
+  if (a.deal && unit < ((u32)a.units & ~7u)) {
     const u32 r = blockIdx.x % (8 * sides);
     unit = blockIdx.x / (8 * sides) * 8 + r % 8, sh = r / 8;
   }
@@ -390,16 +393,16 @@ extern "C" int uwc_kv_append(const void* qkv, int64_t qkv_stride, int dtype, int
   const char* fn = "uwc_kv_append";
   if (int st = check_cache(fn, k, v, ks, vs, pages, page, Hkv, hd, dtype)) return st;
   if (T < 0 || B < 0 || H < 0 || width < 0 || table_stride < 0) return uwc_fail("%s: bad T=%d B=%d H=%d width=%d", fn, T, B, H, width);
-  if (T == 0 || B == 0) return UWC_OK;
-  if (!qkv || !ctx || !table || !cosb || !sinb || (!q && H) || positions <= 0) return uwc_fail("%s: null or empty arguments", fn);
+  if (T == 0) return UWC_OK;
+  if (!qkv || (B && (!ctx || !table)) || !cosb || !sinb || (!q && H) || positions <= 0) return uwc_fail("%s: null or empty arguments", fn);
   if (!cu && T != B) return uwc_fail("%s: without cu every sequence has one row (T=%d B=%d)", fn, T, B);
   if (qkv_stride % 8 || (((uintptr_t)qkv | (uintptr_t)q) & 15))
     return uwc_fail("%s: rows of qkv and q must be 16-byte aligned", fn);
-  const long units = cu ? touched_bound(B, T, page) : B;
+  const long units = B == 0 ? 0 : cu ? touched_bound(B, T, page) : B;
   const long blocks = units * 2 * Hkv + ((H ? (long)T : 0) + 3) / 4;
   if (blocks > 0xFFFFFF) return uwc_fail("%s: too many tokens (%d) and heads (%d)", fn, T, Hkv);  // 2^32 threads
   const AppendArgs a{qkv, qkv_stride, {cu, B, T}, ctx, table, table_stride, width, cosb, sinb, positions, q_norm, k_norm, eps,
-                     H, Hkv, __builtin_ctz((unsigned)page), pages, k, v, ks, vs, q, (int)units};
+                     H, Hkv, __builtin_ctz((unsigned)page), pages, k, v, ks, vs, q, (int)units, T > 4L * B};
   const dim3 grid((unsigned)blocks), wg(256);
 #define KV_APPEND(HD, ROUNDS)                                                                              \
   do {                                                                                                     \

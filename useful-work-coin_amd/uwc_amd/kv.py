@@ -21,7 +21,8 @@ cu[b] .. cu[b + 1] - 1 (int32, cu[0] = 0); without cu every sequence has one, a 
 cu[B] on (a batch padded to a fixed size) belong to no sequence and come out as zeros. 16-bit rows are
 bfloat16 or float16. Index tensors are int32 on the cache's GPU; nothing here reads them on the host, so
 every call can be captured into a graph. A page that a row needs but that is not in the cache (an entry
-outside [0, pages), a position past the table's width) makes that row NaN; nothing else is touched.
+outside [0, pages), a position past the table's width) makes that row NaN; nothing else is touched. Nothing is recorded for autograd: a cache has no
+gradient.
 
 Everything runs on torch's current HIP stream; buffers are torch tensors on the caller's GPU. Arguments
 of the usual form (dense, aligned) take a short way through native code; what follows it in each function
