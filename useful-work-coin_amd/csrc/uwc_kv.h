@@ -37,22 +37,29 @@ struct KvRows {
   int B, T;
 };
 
-__device__ __forceinline__ int kv_new(const KvRows& R, int b) {
-  if (!R.cu) return 1;
-  const int n = R.cu[b + 1] - R.cu[b];
-  return n < 0 ? 0 : n > R.T ? R.T : n;
-}
+// A unit of work: number j of sequence b's, whose new rows are row0 .. row0 + n - 1, and its entry x of the call's
+// per-sequence numbers (tokens cached before, or after).
+struct KvUnit {
+  int b, j, row0, n, x;
+};
 
-// Finds unit number `unit` of the list in which sequence b has count(b) units: its sequence and its index
-// there, uniform over the wave as `unit` has to be. False past the list's end; unit then holds its distance from it.
+// Finds unit number `unit` of the list in which a sequence of n new rows and number x has count(n, x) units, uniform over
+// the wave as `unit` has to be. False past the list's end; unit then holds its distance from it. A sequence's numbers are
+// loaded once, by the lane that counts its units. For packed rows (R.cu).
 template <class F>
-__device__ __forceinline__ bool kv_find(int& unit, int B, F&& count, int& b, int& j) {
+__device__ __forceinline__ bool kv_find(const KvRows& R, const int* xs, int& unit, F&& count, KvUnit& u) {
   const int lane = threadIdx.x & 63;
-  int n = lane < B ? count(lane) : 0;
-  for (int base = 0; base < B; base += 64) {
-    const int next = base + 64 + lane < B ? count(base + 64 + lane) : 0;
+  int c0 = 0, x = 0, n = 0;
+  auto load = [&](int i) KV_AI {
+    if (i >= R.B) return c0 = x = n = 0, 0;
+    c0 = R.cu[i], x = xs[i], n = R.cu[i + 1] - c0;
+    n = n < 0 ? 0 : n > R.T ? R.T : n;
+    return count(n, x);
+  };
+  for (int base = 0; base < R.B; base += 64) {
+    const int units = load(base + lane);
     // the inclusive sums over the lanes: within rows of 16, then of the rows before
-    int s = n;
+    int s = units;
     s += __builtin_amdgcn_update_dpp(0, s, 0x111, 0xf, 0xf, true);  // row_shr:1, :2, :4, :8
     s += __builtin_amdgcn_update_dpp(0, s, 0x112, 0xf, 0xf, true);
     s += __builtin_amdgcn_update_dpp(0, s, 0x114, 0xf, 0xf, true);
@@ -62,12 +69,12 @@ __device__ __forceinline__ bool kv_find(int& unit, int B, F&& count, int& b, int
     const int total = __builtin_amdgcn_readlane(s, 63);
     if (unit < total) {
       const int l = __builtin_ctzll(__ballot(s > unit));
-      b = base + l;
-      j = unit - (__builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(n, l));
+      u.b = base + l;
+      u.j = unit - (__builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(units, l));
+      u.row0 = __builtin_amdgcn_readlane(c0, l), u.n = __builtin_amdgcn_readlane(n, l), u.x = __builtin_amdgcn_readlane(x, l);
       return true;
     }
     unit -= total;
-    n = next;
   }
   return false;
 }

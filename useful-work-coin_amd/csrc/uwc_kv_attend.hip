@@ -124,17 +124,14 @@ struct Unit {
 
 // Unit number u of tiles of M rows; false past the last (u then counts on from there).
 __device__ __forceinline__ bool unit_of(const AttendArgs& a, int& u, int M, Unit& x) {
-  int b, j;
   if (a.rows.cu) {
-    if (!kv_find(u, a.rows.B, [&](int s) KV_AI { return (int)(((long)kv_new(a.rows, s) * a.G + M - 1) / M); }, b, j)) return false;
-    x.row0 = a.rows.cu[b];
+    KvUnit k;
+    if (!kv_find(a.rows, a.lens, u, [&](int n, int) KV_AI { return (int)(((long)n * a.G + M - 1) / M); }, k)) return false;
+    x.b = k.b, x.r0 = k.j * M, x.rows = k.n * a.G, x.row0 = k.row0, x.len = k.x;
   } else {
     const int per = (a.G + M - 1) / M;
-    b = u / per, j = u % per;
-    x.row0 = b;
+    x.b = uniform(u / per), x.r0 = uniform(u % per * M), x.rows = a.G, x.row0 = x.b, x.len = uniform(a.lens[x.b]);
   }
-  x.b = uniform(b), x.r0 = uniform(j * M), x.rows = uniform(kv_new(a.rows, b) * a.G), x.len = uniform(a.lens[b]);
-  x.row0 = uniform(x.row0);
   return true;
 }
 

@@ -147,6 +147,12 @@ __device__ __forceinline__ u32 again4(u32 w, float old, double rd) {
   return r;
 }
 
+// Pages that n tokens from position x on touch.
+__device__ __forceinline__ int pages_of(int n, int x, int lp) {
+  const int P = 1 << lp;
+  return n == 0 || x < 0 ? 0 : (int)(((u32)(n + (x & (P - 1))) + P - 1) >> lp);
+}
+
 // The new tokens of one page of one kv head, keys (SIDE 0) or values (SIDE 1), by one workgroup.
 // ROUNDS rounds of 256 / (hd / 16) tokens cover the page.
 template <int HD, int ROUNDS, int SIDE, class T>
@@ -155,16 +161,13 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, int unit, int h
   __shared__ u32 wmax[4];
   __shared__ __attribute__((aligned(16))) u8 img[SIDE ? HD * (PER * ROUNDS + 16) : 16];
   const int P = 1 << a.lp, tid = threadIdx.x, c = tid % LPH;
-  int b = unit, j = 0;
-  if (a.rows.cu && !kv_find(unit, a.rows.B, [&](int s) KV_AI {
-        const int n = kv_new(a.rows, s), x = a.ctx[s];
-        return n == 0 || x < 0 ? 0 : (int)(((u32)(n + (x & (P - 1))) + P - 1) >> a.lp);
-      }, b, j))
-    return;
-  const int ctx = a.ctx[b], n = kv_new(a.rows, b), lead = ctx & (P - 1);
+  KvUnit u{unit, 0, unit, 1, 0};
+  if (!a.rows.cu) u.x = a.ctx[unit];
+  else if (!kv_find(a.rows, a.ctx, unit, [&](int n, int x) KV_AI { return pages_of(n, x, a.lp); }, u)) return;
+  const int b = u.b, j = u.j, ctx = u.x, n = u.n, lead = ctx & (P - 1);
   if (ctx < 0) return;
   const int first = j ? 0 : lead, i0 = j ? (j << a.lp) - lead : 0;
-  const int row0 = (a.rows.cu ? a.rows.cu[b] : b) + i0;  // row of slot `first`
+  const int row0 = u.row0 + i0;  // row of slot `first`
   int cnt = n - i0 < P - first ? n - i0 : P - first;
   const long id = page_of(a, b, (ctx >> a.lp) + j);
   if (id < 0) return;
@@ -317,15 +320,12 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
   typedef typename kv_vec<T>::v8 v8;
   const int P = 1 << a.lp, tid = threadIdx.x;
   const int h = blockIdx.x % a.Hkv;
-  int unit = blockIdx.x / a.Hkv, b, j;
-  if (!kv_find(unit, a.rows.B, [&](int s) KV_AI {
-        const int n = kv_new(a.rows, s), x = a.start[s];
-        return n == 0 || x < 0 ? 0 : (int)(((u32)(n + (x & (P - 1))) + P - 1) >> a.lp);
-      }, b, j))
-    return;
-  const int start = a.start[b], n = kv_new(a.rows, b), lead = start & (P - 1);
+  int unit = blockIdx.x / a.Hkv;
+  KvUnit u;
+  if (!kv_find(a.rows, a.start, unit, [&](int n, int x) KV_AI { return pages_of(n, x, a.lp); }, u)) return;
+  const int b = u.b, j = u.j, start = u.x, n = u.n, lead = start & (P - 1);
   const int first = j ? 0 : lead, i0 = j ? (j << a.lp) - lead : 0, col = (start >> a.lp) + j;
-  const int row0 = a.rows.cu[b] + i0 - first;  // row of slot 0
+  const int row0 = u.row0 + i0 - first;  // row of slot 0
   int lo = first, hi = first + (n - i0 < P - first ? n - i0 : P - first);
   lo = lo > -row0 ? lo : -row0;
   hi = hi < a.rows.T - row0 ? hi : a.rows.T - row0;
