@@ -148,3 +148,30 @@ def test_other_entries_refuse():
                         (dict(rows=1 << 30, Hkv=64), "too many")):
         st, err = read(**change)
         assert st == -1 and "uwc_kv_read" in err and msg in err, change
+
+
+def test_short_way_is_built_from_this_header_and_declines_other_forms(monkeypatch):
+    """_kv.so carries the header's stamp, returns None for what is not of the usual form (here: not on a GPU) or
+    not as many arguments as it takes, and is refused when it was built from another header."""
+    from uwc_amd import _lib
+    k = _lib.kv()
+    assert k.header_sha() == _lib.lib().uwc_header_sha().decode()
+    cache = cpu_cache()
+    q, table, lens = torch.zeros((1, 4, 64), dtype=BF), torch.zeros((1, 2), dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    assert k.attend(*cache, q, table, lens, None, None, None, 0, 0, None, 0) is None
+    assert k.attend(*cache, q) is None and k.attend() is None
+    assert k.append(1, 2, 3, 4, 5, 6, 7, 8, 9, None, None, None, 1e-6, 0) is None
+    assert k.read(*cache, table, lens, lens, 1, False, 0) is None
+    with pytest.raises(TypeError):
+        k.bind(1)
+
+    class Other:
+        header_sha = staticmethod(lambda: "0" * 16)
+
+    import sys
+    import uwc_amd
+    monkeypatch.setattr(_lib, "_KV", None)
+    monkeypatch.setitem(sys.modules, "uwc_amd._kv", Other)
+    monkeypatch.setattr(uwc_amd, "_kv", Other, raising=False)
+    with pytest.raises(ImportError, match="different include/uwc.h"):
+        _lib.kv()

@@ -424,7 +424,7 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(AttendArgs a) {
 // hit all of its 64 banks: 16 rows of an operand that are read, two key rows or four value rows that are written. K's operand row m is key 16 (m >> 4) + 8 (m >> 2 & 1) + 4 (m >> 3 & 1) +
 // (m & 3) of its 32: the scores of lane half hf are then keys 16 n + 8 hf + i, the 8 k slots of V's product n.
 //
-// Measured: 4096 tokens over 32768, 16 heads of 128, 964 to 1013 us by box = 1070 to 1018 TFLOP/s, at a clock that the
+// Measured: 4096 tokens over 32768, 16 heads of 128, 964 to 1031 us by box = 1070 to 1000 TFLOP/s, at a clock that the
 // load drives down to about 1.88 GHz (an fp16 product of 16384^3 reaches 1263 to 1328 here): matrix units busy 53% of its
 // cycles, VALU 60%. 6000 tokens under a window of 1024, heads of 64: 47 us, the weights' VALU work (three workgroups to a
 // CU, 168 registers; two 58 us).
