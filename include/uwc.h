@@ -419,7 +419,7 @@ int uwc_sha_merkle_roots(const uint32_t* leaves, int ntrees, int n, uint32_t* sc
  * (its DetQwen3.generate_greedy keeps whole fp32 rows, runtime/detrt/qwen3.py:296-334).
  *
  * One layer's cache: k int8 (pages, Hkv, page, hd); v int8 (pages, Hkv, hd, page), tokens innermost; ks, vs
- * fp32 (pages, Hkv), the scale of a page's keys and values of one head. page is 16, 32, 64 or 128, hd 32,
+ * fp32 (pages, Hkv), the scale (not negative) of a page's keys and values of one head. page is 16, 32, 64 or 128, hd 32,
  * 64 or 128; k and v 16-byte aligned. Token p of sequence b lies in slot p % page of page
  * table[b * table_stride + p / page]; a row of the table has `width` entries, those past a sequence's pages
  * are not read.
@@ -445,8 +445,8 @@ int uwc_kv_append(const void* qkv, int64_t qkv_stride, int dtype, int T, int B, 
 
 /* o (T, H, hd) = causal attention of q (T tokens, q_stride elements apart, H heads of hd) over the cache:
  * sequence b has lens[b] tokens in it, its queries are the last of them. window > 0: a query at position p
- * sees keys above p - window, and those below `sinks`. Scores are scaled by `scale`. Rows that see nothing
- * are zeros. max_new and max_len (0: unknown) bound the sequences' new tokens and lengths: they choose how
+ * sees keys above p - window, and those below `sinks`. Scores are scaled by `scale` > 0. Rows that see
+ * nothing are zeros. max_new and max_len (0: unknown) bound the sequences' new tokens and lengths: they choose how
  * the work is split, and results are right for any. scratch: uwc_kv_attend_scratch_bytes bytes, 16-byte
  * aligned, no contents kept between calls (may be NULL when that is 0). Sums and softmax statistics are fp32,
  * probabilities are rounded to fp16 for the product with the values. */

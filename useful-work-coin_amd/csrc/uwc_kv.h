@@ -14,7 +14,6 @@
 #define KV_AI __attribute__((always_inline))
 
 typedef _Float16 h2v __attribute__((ext_vector_type(2)));
-typedef _Float16 h4v __attribute__((ext_vector_type(4)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef __bf16 b8v __attribute__((ext_vector_type(8)));
 typedef u32 u4v __attribute__((ext_vector_type(4)));

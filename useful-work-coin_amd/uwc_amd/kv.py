@@ -153,7 +153,7 @@ def attend(cache, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, cu=N
     them. H is a multiple of the cache's Hkv; q head i reads kv head i // (H / Hkv). window > 0: a query at
     position p sees keys above p - window, and the sequence's first `sinks`. Rows that see nothing are zeros.
     max_new, max_len: bounds of the sequences' new tokens and lengths that the caller knows, for splitting
-    the work well; results are right for any. scale defaults to 1 / sqrt(hd)."""
+    the work well; results are right for any. scale, above 0, defaults to 1 / sqrt(hd)."""
     r = _lib.kv().attend(*cache, q, table, lens, cu, max_new, max_len, window, sinks, scale, _stream())
     if r is not None:
         return r if type(r) is not int else _lib.fail("uwc_kv_attend", r)
