@@ -415,9 +415,9 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(AttendArgs a) {
 // scores (32 matrix instructions, 1024 cycles, fed by LDS reads six ahead), between which the next bytes are
 // converted, written to LDS and loaded. With eight waves the two of a SIMD take turns at the halves, a barrier apart.
 //
-// Four waves (two workgroups to a CU) keep two stages of keys and of values: the keys of tile i + 2 are written in
-// the second half of step i, when keys i are done with and keys i + 1 are read; the values of tile i + 1 in the first half of
-// step i, when values i - 1 are done with. Eight waves keep four stages of either, as the waves that are half a
+// Four waves (two workgroups to a CU) keep two stages of keys and of values: in the second half of step i, which reads
+// keys i + 1 and values i, the keys of tile i + 2 take the place of keys i and the values of tile i + 1 that of values
+// i - 1, both last read before the barriers between. Eight waves keep four stages of either, as the waves that are half a
 // step behind still read values i when the others are a half past them, and write tile i + 2 in step i's second half.
 //
 // LDS rows hold 16-byte pieces (8 fp16), piece c of row r at c ^ swz(r), such that 16 lanes, which LDS serves at once,
@@ -680,13 +680,6 @@ __global__ __launch_bounds__(64 * NW, HD <= 64 ? 3 : 2) void kv_attend_many_kern
         if (S == 0 && i % 16 == 4) load_scales(next);
         if (S == 0 && i % 16 == 8) put_granule(i + 8, next);
       }
-      if (!TURNS)
-#pragma unroll
-        for (int k = 0; k < PER; k++)
-          if (of_values(k)) {
-            half_to_lds(S + 1, k, 0), half_to_lds(S + 1, k, 1);
-            load_piece(i + 2, k);
-          }
       const int key0 = sp.tile(t0 + i) * 64;
       softmax_tile<DB>(a, s, A, pos, all_seen(a, of_wave, key0, 64), key0 + 8 * hf, meta[i & 31], o, mr, l, p);
       __builtin_amdgcn_sched_barrier(0);
@@ -698,8 +691,8 @@ __global__ __launch_bounds__(64 * NW, HD <= 64 ? 3 : 2) void kv_attend_many_kern
       for (int k = 0; k < PRE; k++) f[k] = frag(S, k);
       __builtin_amdgcn_sched_barrier(0);
       // Between the products, a part at a time: step i + 2's pieces into LDS, step i + 3's loads, the pages for the
-      // loads after those (four waves: of the keys; the values' turn is above). What is past the last tile is for nothing.
-      constexpr int MINE = !TURNS && PER > 1 ? PER / 2 : PER, PARTS = 3 * MINE + 1;
+      // loads after those (four waves: of the values each a step nearer). What is past the last tile is for nothing.
+      constexpr int PARTS = 3 * PER + 1;
 #pragma unroll
       for (int k = 0; k < NP; k++) {
         product(k, f[k % PRE]);
@@ -711,9 +704,10 @@ __global__ __launch_bounds__(64 * NW, HD <= 64 ? 3 : 2) void kv_attend_many_kern
               if (j == PARTS - 1) {
 #pragma unroll
                 for (int c = 0; c < PER; c++) load_id(!TURNS && of_values(c) ? i + 3 : i + 4, c);
-              } else if (TURNS || !of_values(j / 3)) {
-                if (j % 3 == 2) load_piece(i + 3, j / 3);
-                else half_to_lds(S + 2, j / 3, j % 3);
+              } else {
+                const int nearer = !TURNS && of_values(j / 3);
+                if (j % 3 == 2) load_piece(i + 3 - nearer, j / 3);
+                else half_to_lds(S + 2 - nearer, j / 3, j % 3);
               }
             }
         __builtin_amdgcn_sched_barrier(0);
