@@ -224,6 +224,17 @@ def test_attend_eight_waves(dev, new, lens, dtype):
     check(kv.attend(cache, q, table, L, cu=cu, max_new=max(new), max_len=max(lens)), want, tol)
 
 
+@pytest.mark.parametrize("new,lens,H,Hkv,window,sinks", [([300], [3001], 4, 1, 0, 0), ([300], [3001], 4, 1, 1000, 70), ([300, 1, 257], [900, 1000, 4000], 16, 4, 0, 0),
+                                                         ([140, 129], [140, 5000], 14, 2, 2048, 5), ([2070, 2100], [2100, 5000], 16, 16, 2048, 4)])
+def test_attend_eight_waves_over_a_context(dev, new, lens, H, Hkv, window, sinks):
+    """256 rows to a workgroup where most keys are earlier ones, with and without windows, and in split parts."""
+    from uwc_amd import kv
+    cache, q, table, L, cu = problem(dev, new, lens, H, Hkv, 128, 64, BF, seed=len(new) + H)
+    want, tol = R.attend(cache, q, table, L, cu, window, sinks)
+    check(kv.attend(cache, q, table, L, cu=cu, max_new=max(new), max_len=max(lens), window=window, sinks=sinks), want, tol)
+    check(kv.attend(cache, q, table, L, cu=cu, max_new=max(new), max_len=1 << 16, window=window, sinks=sinks), want, tol, "high bound")
+
+
 def test_short_and_long_way_agree(dev, monkeypatch):
     """The native way for arguments of the usual form and the one that looks at any: the same bits."""
     from uwc_amd import _lib, kv

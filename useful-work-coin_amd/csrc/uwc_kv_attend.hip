@@ -796,7 +796,8 @@ Plan plan_of(int T, int B, bool packed, int H, int Hkv, int hd, int max_new, int
   Plan p;
   const int G = H / Hkv;
   const long cus = uwc_cu_count(), rows = (long)(packed ? (max_new > 0 && max_new < T ? max_new : T) : 1) * G;
-  long keys = max_len > 0 ? max_len : 1;
+  const long keys_all = max_len > 0 ? max_len : 1;
+  long keys = keys_all;
   if (window && (long)window + sinks + rows / G + 64 < keys) keys = (long)window + sinks + rows / G + 64;
   const long tiles = (keys + 63) / 64;
   // Tiles of 16 rows while at most 80 of them per CU meet a tile of 64 keys (40 of more than 128 rows): they spread best,
@@ -805,10 +806,13 @@ Plan plan_of(int T, int B, bool packed, int H, int Hkv, int hd, int max_new, int
   // 8000, 16 sequences 122 / 98), two tiles of 16 to a wave for heads of 64 and fewer, whose keys cost less to read
   // than to convert (300 tokens of 16 heads, 600 rows, 10 / 16, 1000 of them 50 / 33; 5 tokens of 7 heads to a kv head of 64, 8 x 20000: 92 -> 67, many 74; heads of 128: 78.6 / 78.2).
   const bool light = (rows + 15) / 16 * B * Hkv * tiles <= (rows <= 128 ? 80 : 40) * cus;
-  // Many: 256 rows share a tile's conversion where that still fills the CUs, 128 rows leave less idle where not (us, 256 /
-  // 128 rows: 4096 tokens over 32768, 2 heads to a kv head of 128, 985 / 1116; ragged prompts up to 777, 60 / 24; 6000
-  // tokens under a window of 1024, 4 heads of 64, 76 / 59).
-  const bool wide = hd == 128 && !window && (long)T * G / 256 * Hkv >= cus;
+  // Many: heads of 128 may take 256 rows to a tile, which share its conversion (4096 tokens over 32768, 2 heads to a kv
+  // head, 985 us, 128 rows 1070). 128 rows leave less idle where tiles differ much in length and do not fill
+  // the CUs (a prompt of 2000, 4 heads to a kv head, 256 / 128 rows 62 / 56; 512 tokens over 8000 88 / 93, over
+  // 30000 256 / 280), where a short window leaves more of a tile's keys to few of 256 rows (8000 tokens, windows of 1000 183 / 178, 2000
+  // 292 / 291, 4000 412 / 438), and where sequences have fewer rows than that (16 of up to 100 tokens 187 / 171).
+  const bool filled = (long)T * G / 256 * Hkv >= cus;
+  const bool wide = hd == 128 && (long)T * G >= 256L * B && (filled ? !window || window >= 2048 : keys_all * G >= 3 * rows);
   p.form = light || rows <= 16 ? KV_FEW1 : hd <= 64 && rows <= 48 ? KV_FEW2 : rows <= 32 ? KV_FEW1 : wide ? KV_MANY8 : KV_MANY4;
   p.m = p.form == KV_FEW1 ? 16 : p.form == KV_FEW2 ? 32 : p.form == KV_MANY4 ? 128 : 256;
   const int M = p.m;
