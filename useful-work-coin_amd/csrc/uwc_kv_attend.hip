@@ -533,14 +533,14 @@ __global__ __launch_bounds__(64 * NW, HD <= 64 ? 3 : 2) void kv_attend_many_kern
   // that starts 16 tiles, the scales some steps later, and when 8 are left both are put into LDS for the next 16.
   const int* const pages_of = a.table + x.b * a.table_stride;
   struct Granule {
-    int page;  // -2: nobody looks
+    int page;  // -1: needed and not there; -2: nobody looks
     float ks, vs;
   };
   auto load_page = [&](int t, Granule& c) KV_AI {
     t += lane >> 2;
     const int key0 = sp.tile(t0 + t) * 64 + 16 * (lane & 3), col = key0 >> a.lp;
     c.page = -2;
-    if (t < n && any_seen(a, sp, key0, 16)) c.page = col < a.width ? pages_of[col] : -1;
+    if (t < n && any_seen(a, sp, key0, 16)) c.page = col < a.width ? max(pages_of[col], -1) : -1;
   };
   auto load_scales = [&](Granule& c) KV_AI {
     c.page = c.page < a.pages ? c.page : -1;
