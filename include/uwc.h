@@ -449,7 +449,8 @@ int uwc_kv_append(const void* qkv, int64_t qkv_stride, int dtype, int T, int B, 
  * nothing are zeros. max_new and max_len (0: unknown) bound the sequences' new tokens and lengths: they choose how
  * the work is split, and results are right for any. scratch: uwc_kv_attend_scratch_bytes bytes, 16-byte
  * aligned, no contents kept between calls (may be NULL when that is 0). Sums and softmax statistics are fp32,
- * probabilities are rounded to fp16 for the product with the values. */
+ * probabilities times the values' scales are rounded to fp16 for the product with the values' bytes: each is off by at
+ * most 2^-11 of itself, or 2^-32 of the row's largest where that is more. */
 uint64_t uwc_kv_attend_scratch_bytes(int T, int B, int packed, int H, int Hkv, int hd, int max_new, int max_len,
                                      int window, int sinks);
 int uwc_kv_attend(const int8_t* k, const int8_t* v, const float* ks, const float* vs, int64_t pages, int page, int Hkv,

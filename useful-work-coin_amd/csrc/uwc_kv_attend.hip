@@ -18,8 +18,11 @@
 // by lane, the operand of O^T = V^T P^T; P never leaves them. The keys of a tile are dealt to the rows of K's
 // operand so that a lane gets 16 consecutive tokens: one granule, one scale, one 16-byte piece of V's rows.
 //
-// The running maximum m only moves when some row's new maximum exceeds it by 2^8 or more (w then stays below
-// 2^9, far inside fp16), so that most tiles neither exchange maxima between lanes nor rescale O.
+// m is not the row's maximum itself but at least 7 below it, and it only moves when some row's new maximum exceeds it by
+// more than 15: the largest w lies in [2^7, 2^15], near the top of fp16, and most tiles neither exchange maxima between
+// lanes nor rescale O. Weights down to 2^-21 of the row's largest then keep fp16's 11 bits, smaller ones are off by at most 2^-32
+// of it: the long flat tail behind one key that is far ahead (a first token that all rows look at, often with values
+// near 0) still counts. With the largest w at 1, 9000 keys 18 nats behind one of value 0 came out as 0.
 #include <type_traits>
 
 #include "uwc_kv.h"
@@ -49,7 +52,7 @@ struct AttendArgs {
 };
 
 constexpr float KV_LOWEST = -3e38f;  // m of a row that has seen nothing: differences from it stay numbers
-constexpr float KV_SLACK = 8.0f;
+constexpr float KV_BELOW = 7.0f, KV_MOVE = 15.0f;
 
 // bytes of w as four fp16: 0x6400 | (x + 128) is 1024 + x + 128 in fp16, and subtracting 1152 is exact
 __device__ __forceinline__ void to_half4(u32 w, h2v& a, h2v& b) {
@@ -343,8 +346,8 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(AttendArgs a) {
       }
 #pragma unroll
       for (int i = 0; i < 16; i++) top = fmaxf(top, e[i]);
-      if (__any(top > mr[rb] + KV_SLACK)) {
-        const float to = fmaxf(mr[rb], max_xor32(max_xor16(top)));
+      if (__any(top > mr[rb] + KV_MOVE)) {
+        const float to = fmaxf(mr[rb], max_xor32(max_xor16(top)) - KV_BELOW);
         const float f = __builtin_amdgcn_exp2f(mr[rb] - to);
         mr[rb] = to;
         l[rb] *= f;
@@ -467,8 +470,8 @@ __device__ __forceinline__ void softmax_tile(const AttendArgs& a, f16v s[2], flo
     for (int i = 1; i < 8; i++) g = fmaxf(g, s[n >> 1][8 * (n & 1) + i]);
     top = fmaxf(top, __builtin_fmaf(g, Ak[n], lk[n]));
   }
-  if (__any(top > mr + KV_SLACK)) {
-    const float to = fmaxf(mr, max_xor32(top));
+  if (__any(top > mr + KV_MOVE)) {
+    const float to = fmaxf(mr, max_xor32(top) - KV_BELOW);
     const float f = __builtin_amdgcn_exp2f(mr - to);
     mr = to;
     l *= f;
