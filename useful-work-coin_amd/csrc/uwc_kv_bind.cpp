@@ -81,7 +81,7 @@ bool cache_of(Look& L, PyObject* const* a, Cache& c) {
   if (!L.ok) return false;
   const int64_t n = k->size(0), H = k->size(1), P = k->size(2), D = k->size(3);
   if (v->size(0) != n || v->size(1) != H || v->size(2) != D || v->size(3) != P || ks->size(0) != n || ks->size(1) != H ||
-      vs->size(0) != n || vs->size(1) != H || H > 65535 || P > 128 || D > 128)
+      vs->size(0) != n || vs->size(1) != H || n < 1 || H < 1 || H > 65535 || P < 1 || P > 128 || D < 1 || D > 128)
     return L.ok = false;
   c = Cache{k->data_ptr<int8_t>(), v->data_ptr<int8_t>(), ks->data_ptr<float>(), vs->data_ptr<float>(), n, (int)P, (int)H, (int)D};
   return true;

@@ -69,6 +69,8 @@ def _cache(fn, cache):
             or ks.shape != (n, Hkv) or vs.shape != (n, Hkv)):
         raise AssertionError(f"{fn}: the cache is int8 k (pages, Hkv, page, hd) and v (pages, Hkv, hd, page), float32 ks and "
                              f"vs (pages, Hkv); got {[(tuple(x.shape), x.dtype) for x in cache]}")
+    if not k.numel():
+        raise AssertionError(f"{fn}: the cache is empty, k {tuple(k.shape)}")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise AssertionError(f"{fn}: the cache's tensors must be contiguous")
     return k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), n, page, Hkv, hd
