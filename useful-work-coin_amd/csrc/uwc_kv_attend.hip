@@ -918,7 +918,7 @@ extern "C" int uwc_kv_attend(const int8_t* k, const int8_t* v, const float* ks, 
     return uwc_fail("%s: scratch holds %llu bytes, %llu needed", fn, (unsigned long long)(scratch ? scratch_bytes : 0),
                     (unsigned long long)p.bytes);
   const long blocks = p.units * p.splits * Hkv;
-  if (blocks > 0xFFFFFF) return uwc_fail("%s: too many tokens (%d) and heads (%d)", fn, T, H);  // 2^32 threads
+  if (blocks * (p.form == KV_MANY8 ? 512 : 256) > 0xFFFFFFFF) return uwc_fail("%s: too many tokens (%d) and heads (%d)", fn, T, H);
   AttendArgs a{k, v, ks, vs, pages, q, q_stride, table, table_stride, width, lens, {cu, B, T}, H, Hkv, H / Hkv,
                __builtin_ctz((unsigned)page), window, sinks, scale * 1.4426950408889634f, (int)p.units, p.splits, p.tps, blocks <= 2L * uwc_cu_count(), o,
                static_cast<float*>(scratch), reinterpret_cast<float2*>(static_cast<char*>(scratch) + p.o_bytes)};
