@@ -427,7 +427,8 @@ int uwc_sha_merkle_roots(const uint32_t* leaves, int ntrees, int n, uint32_t* sc
  * means one row each (T = B). Rows from cu[B] on belong to no sequence: their outputs are zeros.
  * 16-bit rows are UWC_KV_BF16 or UWC_KV_FP16. Device-side numbers cannot be refused by a return value: a
  * page that is needed but outside [0, pages) or past the table's width, or a position past the rotation
- * tables, makes the rows that need it NaN, and nothing outside the buffers is read or written. */
+ * tables, makes the rows that need it NaN, a negative ctx or start all rows of its sequence, and nothing outside the
+ * buffers is read or written. */
 #define UWC_KV_BF16 0
 #define UWC_KV_FP16 1
 
@@ -460,7 +461,7 @@ int uwc_kv_attend(const int8_t* k, const int8_t* v, const float* ks, const float
                   hipStream_t stream);
 
 /* Tokens start[b] .. start[b] + cu[b + 1] - cu[b] - 1 of every sequence as values, z s rounded once:
- * ko, vo (rows, Hkv, hd). Rows from cu[B] on are not written. */
+ * ko, vo (rows, Hkv, hd), rows at least cu[B]. */
 int uwc_kv_read(const int8_t* k, const int8_t* v, const float* ks, const float* vs, int64_t pages, int page, int Hkv,
                 int hd, const int32_t* table, int64_t table_stride, int width, const int32_t* start, const int32_t* cu,
                 int B, int rows, int dtype, void* ko, void* vo, hipStream_t stream);

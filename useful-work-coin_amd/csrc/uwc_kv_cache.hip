@@ -8,7 +8,7 @@
 //           with max over the page's new tokens; where it holds older ones s is at least their scale, and
 //           they are rounded again, rint(z old / s), if it grew. An unchanged scale leaves them as they are
 //           (rint(z s / s) = z), so a decode step writes its token alone.
-//   read    value = z s of a range of tokens, rounded once to the output type.
+//   read    value = z s of a range of tokens, rounded once to the output type; zeros in rows of no sequence.
 //
 // Bytes bound both where tokens are many (a prefill of 3890 tokens, 16 + 2 x 8 heads of 128: 60 MB in 15.8 us; 30000 tokens
 // read back, 184 MB in 36.0 us, 5.1 TB/s), the chain cu -> table -> rows -> scale where they are few (one token 4.0 us,
@@ -313,7 +313,8 @@ struct ReadArgs {
   void *ko, *vo;
 };
 
-// One page's tokens of one kv head. The first (HD / 8) (P / 16) pieces of work are its values', 16 tokens of 8 dims
+// One page's tokens of one kv head; of a sequence that starts below 0 as many NaN. Workgroups past the last page take a
+// page's worth of the rows of no sequence each, zeros. The first (HD / 8) (P / 16) pieces of work are its values', 16 tokens of 8 dims
 // each: 16-byte loads along the tokens, 16-byte stores along the dims; the others its keys', 16 dims of a token.
 template <int HD, class T>
 __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
@@ -322,14 +323,23 @@ __global__ __launch_bounds__(256) void kv_read_kernel(ReadArgs a) {
   const int h = blockIdx.x % a.Hkv;
   int unit = blockIdx.x / a.Hkv;
   KvUnit u;
-  if (!kv_find(a.rows, a.start, unit, [&](int n, int x) KV_AI { return pages_of(n, x, a.lp); }, u)) return;
-  const int b = u.b, j = u.j, start = u.x, n = u.n, lead = start & (P - 1);
+  if (!kv_find(a.rows, a.start, unit, [&](int n, int x) KV_AI { return pages_of(n, x < 0 ? 0 : x, a.lp); }, u)) {
+    const int from = a.rows.B && a.rows.cu[a.rows.B] > 0 ? a.rows.cu[a.rows.B] : 0;
+    for (int q = tid; q < P * (HD / 8); q += 256) {
+      const long r = from + ((long)unit << a.lp) + q / (HD / 8), at = (r * a.Hkv + h) * HD + q % (HD / 8) * 8;
+      if (r >= a.rows.T) break;
+      store16(static_cast<T*>(a.ko) + at, u4v{0, 0, 0, 0});
+      store16(static_cast<T*>(a.vo) + at, u4v{0, 0, 0, 0});
+    }
+    return;
+  }
+  const int b = u.b, j = u.j, start = u.x < 0 ? 0 : u.x, n = u.n, lead = start & (P - 1);
   const int first = j ? 0 : lead, i0 = j ? (j << a.lp) - lead : 0, col = (start >> a.lp) + j;
   const int row0 = u.row0 + i0 - first;  // row of slot 0
   int lo = first, hi = first + (n - i0 < P - first ? n - i0 : P - first);
   lo = lo > -row0 ? lo : -row0;
   hi = hi < a.rows.T - row0 ? hi : a.rows.T - row0;
-  long id = col < a.width ? a.table[b * a.table_stride + col] : -1;
+  long id = u.x >= 0 && col < a.width ? a.table[b * a.table_stride + col] : -1;
   const bool bad = id < 0 || id >= a.pages;
   if (bad) id = 0;
   const long head = id * a.Hkv + h;
@@ -426,10 +436,11 @@ extern "C" int uwc_kv_read(const int8_t* k, const int8_t* v, const float* ks, co
   const char* fn = "uwc_kv_read";
   if (int st = check_cache(fn, k, v, ks, vs, pages, page, Hkv, hd, dtype)) return st;
   if (rows < 0 || B < 0 || width < 0 || table_stride < 0) return uwc_fail("%s: bad rows=%d B=%d width=%d", fn, rows, B, width);
-  if (rows == 0 || B == 0) return UWC_OK;
-  if (!table || !start || !cu || !ko || !vo) return uwc_fail("%s: null arguments", fn);
+  if (rows == 0) return UWC_OK;
+  if ((B && (!table || !start || !cu)) || !ko || !vo) return uwc_fail("%s: null arguments", fn);
   if (((uintptr_t)ko | (uintptr_t)vo) & 15) return uwc_fail("%s: outputs must be 16-byte aligned", fn);
-  const long blocks = touched_bound(B, rows, page) * Hkv;
+  // one more than the sequences touch: what they leave of the bound may be a part of a page short of the other rows
+  const long blocks = (touched_bound(B, rows, page) + 1) * Hkv;
   if (blocks > 0xFFFFFF) return uwc_fail("%s: too many tokens (%d) and heads (%d)", fn, rows, Hkv);
   const ReadArgs a{k, v, ks, vs, pages, table, table_stride, width, start, {cu, B, rows}, Hkv, __builtin_ctz((unsigned)page), ko, vo};
   const dim3 grid((unsigned)blocks), wg(256);

@@ -21,7 +21,8 @@ cu[b] .. cu[b + 1] - 1 (int32, cu[0] = 0); without cu every sequence has one, a 
 cu[B] on (a batch padded to a fixed size) belong to no sequence and come out as zeros. 16-bit rows are
 bfloat16 or float16. Index tensors are int32 on the cache's GPU; nothing here reads them on the host, so
 every call can be captured into a graph. A page that a row needs but that is not in the cache (an entry
-outside [0, pages), a position past the table's width) makes that row NaN; nothing else is touched. Nothing is recorded for autograd: a cache has no
+outside [0, pages), a position past the table's width) makes that row NaN, and a sequence whose ctx or start
+is negative all of its rows; nothing else is touched. Nothing is recorded for autograd: a cache has no
 gradient.
 
 Everything runs on torch's current HIP stream; buffers are torch tensors on the caller's GPU. Arguments
@@ -191,8 +192,7 @@ def attend(cache, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, cu=N
 
 def read(cache, table: torch.Tensor, start: torch.Tensor, cu: torch.Tensor, rows: int, dtype=torch.bfloat16):
     """Cached tokens as values: keys and values (rows, Hkv, hd) of `dtype`, sequence b's tokens
-    start[b] .. start[b] + cu[b + 1] - cu[b] - 1 at rows cu[b] .. cu[b + 1] - 1. rows is cu[B]; rows past it
-    are not written."""
+    start[b] .. start[b] + cu[b + 1] - cu[b] - 1 at rows cu[b] .. cu[b + 1] - 1. rows is at least cu[B]."""
     if dtype in _TYPES:
         r = _lib.kv().read(*cache, table, start, cu, rows, _TYPES[dtype], _stream())
         if r is not None:
