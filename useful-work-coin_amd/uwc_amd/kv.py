@@ -77,6 +77,11 @@ def _cache(fn, cache):
     return k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), n, page, Hkv, hd
 
 
+def _on_gpu(fn, dev):
+    if dev.type != "cuda":
+        raise AssertionError(f"{fn}: the cache must be on a GPU, got {dev}")
+
+
 def _index(fn, name, x, n, dev):
     if x.dtype != torch.int32 or x.dim() != 1 or x.shape[0] != n or x.device != dev:
         raise AssertionError(f"{fn}: {name} must be int32 ({n},) on the cache's GPU, got {x.dtype} {tuple(x.shape)} on {x.device}")
@@ -140,6 +145,7 @@ def append(cache, qkv: torch.Tensor, table: torch.Tensor, ctx: torch.Tensor, cos
     positions = cos.shape[0]
     cos, sin = _f32(fn, "cos", cos, (positions, hd), dev), _f32(fn, "sin", sin, (positions, hd), dev)
     q_norm, k_norm = _f32(fn, "q_norm", q_norm, (hd,), dev), _f32(fn, "k_norm", k_norm, (hd,), dev)
+    _on_gpu(fn, dev)
     q = torch.empty((T, H, hd), dtype=qkv.dtype, device=dev)
     _lib.call("uwc_kv_append", qkv.data_ptr(), qkv.stride(0), _TYPES[qkv.dtype], T, B, None if cu is None else cu.data_ptr(),
               ctx.data_ptr(), table.data_ptr(), table.stride(0), width, cos.data_ptr(), sin.data_ptr(), positions,
@@ -180,6 +186,7 @@ def attend(cache, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, cu=N
     max_new = most if max_new is None else max(1, min(max_new, most))
     max_len = min(width * page if max_len is None else max(1, max_len), _I32MAX)
     window, sinks = min(window, _I32MAX), min(sinks, _I32MAX)
+    _on_gpu(fn, dev)
     o = torch.empty((T, H, hd), dtype=q.dtype, device=dev)
     need = _lib.lib().uwc_kv_attend_scratch_bytes(T, B, int(cu is not None), H, Hkv, hd, max_new, max_len, window, sinks)
     scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
@@ -205,6 +212,7 @@ def read(cache, table: torch.Tensor, start: torch.Tensor, cu: torch.Tensor, rows
     table = _table(fn, table, dev)
     B, width = table.shape
     start, cu = _index(fn, "start", start, B, dev), _index(fn, "cu", cu, B + 1, dev)
+    _on_gpu(fn, dev)
     ko = torch.empty((rows, Hkv, hd), dtype=dtype, device=dev)
     vo = torch.empty((rows, Hkv, hd), dtype=dtype, device=dev)
     _lib.call("uwc_kv_read", k, v, ks, vs, pages, page, Hkv, hd, table.data_ptr(), table.stride(0), width, start.data_ptr(),
