@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes
 import hashlib
 import os
+import warnings
 
 import torch
 
@@ -138,17 +139,31 @@ def fail(name: str, st: int) -> None:
 _KV = None
 
 
+class _LongWay:
+    """Stands in for _kv.so: every call is left to what follows it in kv.py."""
+
+    @staticmethod
+    def append(*args):
+        return None
+
+    attend = read = append
+
+
 def kv():
     """_kv.so (uwc_kv_bind.cpp), the short way to the key/value cache's entry points, bound to the
-    library; it has to be built from the same header."""
+    library; it has to be built from the same header. Where it is not built or does not fit this torch, calls go
+    through ctypes."""
     global _KV
     if _KV is None:
         L = lib()
         try:
             from . import _kv
         except ImportError as e:
-            raise ImportError(f"{os.path.join(_HERE, '_kv.so')} is not built or does not fit this torch: run "
-                              "useful-work-coin_amd/csrc/build.sh (or __graft_entry__.build())") from e
+            warnings.warn(f"{os.path.join(_HERE, '_kv.so')} is not built or does not fit this torch ({e}): calls of uwc_amd.kv "
+                          "take some 10 us longer each. To build it, run useful-work-coin_amd/csrc/build.sh "
+                          "(or __graft_entry__.build())", RuntimeWarning, stacklevel=3)
+            _KV = _LongWay
+            return _KV
         if _kv.header_sha() != L.uwc_header_sha().decode():
             raise ImportError("_kv.so and libuwc_hip.so were built from different include/uwc.h: rebuild with "
                               "useful-work-coin_amd/csrc/build.sh (or __graft_entry__.build())")
