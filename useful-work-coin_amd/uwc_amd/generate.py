@@ -27,9 +27,25 @@ def _qkv(att):
     return lambda x: torch.cat([att.q_proj(x), att.k_proj(x), att.v_proj(x)], -1)
 
 
+def _rotation(rotary, n: int, dev):
+    """cos and sin (n, head_dim) of positions 0 .. n - 1, for sequences of any length up to n: the rotation must not
+    depend on the length, as that of dynamic and long-context scalings does past the length a model was trained at."""
+    def table(n):
+        cos, sin = rotary(torch.zeros(1, dtype=torch.float32, device=dev), torch.arange(n, device=dev)[None])
+        return cos[0].float().contiguous(), sin[0].float().contiguous()
+
+    whole = table(n)
+    few = table(min(n, 2))  # also leaves the module as short sequences want it
+    if not all(torch.allclose(a[:2], b, rtol=1e-4, atol=0.0) for a, b in zip(whole, few)):
+        raise AssertionError(f"PagedGenerator: the model's rotation at {n} positions is another than that of short sequences; "
+                             "give `positions` up to which it stays the same")
+    return whole
+
+
 class PagedGenerator:
     """The layers of `model` over caches of `pages` pages of `page` tokens each, shared by all sequences.
-    positions: rows of the rotation tables (the model's own limit by default)."""
+    positions: rows of the rotation tables (the model's own limit by default), the longest that a sequence may get; a
+    model whose rotation depends on the length up to there is refused."""
 
     def __init__(self, model, pages: int, page: int = 64, positions: int | None = None):
         cfg = model.config
@@ -41,9 +57,7 @@ class PagedGenerator:
         self.caches = [kv.new_cache(pages, self.Hkv, self.hd, page, dev) for _ in model.model.layers]
         self.free = list(range(pages))
         self.positions = positions or cfg.max_position_embeddings
-        cos, sin = model.model.rotary_emb(torch.zeros(1, dtype=torch.float32, device=dev),
-                                          torch.arange(self.positions, device=dev)[None])
-        self.cos, self.sin = cos[0].float().contiguous(), sin[0].float().contiguous()
+        self.cos, self.sin = _rotation(model.model.rotary_emb, self.positions, dev)
         self.layers = []
         for layer in model.model.layers:
             att = layer.self_attn
