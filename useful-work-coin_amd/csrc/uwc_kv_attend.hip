@@ -191,7 +191,8 @@ __device__ __forceinline__ void zero_rows(const AttendArgs& a, int u, int M, int
 // against 350 VALU and 32 matrix instructions of a wave, a quarter of what its SIMD could do meanwhile, and two
 // workgroups to a CU keep 128 KiB on their way (the next tile's keys are loaded when this one's are used up, its values
 // after the products). 48 sequences of 1500 to 12000 tokens, 8 kv heads of 128: 723 MB in 146 us, 4.96 TB/s; one of
-// 131072: 268 MB in 54, 4.94, the join included. Loads past the caches: 151 and 59.
+// 131072: 268 MB in 54, 4.94, the join included; a copy of 4 GiB moves 4.8 here, a streaming sum of rows reads 6.45. Loads
+// past the caches: 151 and 59.
 template <int HD>
 struct Tile {
   static constexpr int KC = HD >= 64 ? HD / 64 : 1;  // 16-byte pieces (8-byte at HD = 32) of a key row in a lane
@@ -428,9 +429,10 @@ __global__ __launch_bounds__(256) void kv_attend_few_kernel(AttendArgs a) {
 // (m & 3) of its 32: the scores of lane half hf are then keys 16 n + 8 hf + i, the 8 k slots of V's product n.
 //
 // Measured: 4096 tokens over 32768, 16 heads of 128, 964 to 1031 us by box = 1070 to 1000 TFLOP/s, at a clock that the
-// load drives down to about 1.88 GHz (an fp16 product of 16384^3 reaches 1263 to 1328 here): matrix units busy 53% of its
-// cycles, VALU 60%. 6000 tokens under a window of 1024, heads of 64: 47 us, the weights' VALU work (three workgroups to a
-// CU, 168 registers; two 58 us).
+// load drives down to about 1.88 GHz (an fp16 product of 16384^3 reaches 1263 to 1328 here): matrix units busy 52% of its
+// cycles, VALU 59%. 6000 tokens under a window of 1024, heads of 64: 47 us (three workgroups to a CU, 168 registers; two
+// 58 us); neither unit is full, VALU 50% and matrix units 20% of the cycles, with 1.75 waves to a SIMD on average of the
+// three that fit: waves that wait at the barriers, and workgroups that have ended while others go on.
 __device__ __forceinline__ int key_row(int key) { return (key & ~12) | ((key & 4) << 1) | ((key & 8) >> 1); }
 template <int HD>
 __device__ __forceinline__ int k_piece(int r, int c) {  // of rows of HD fp16

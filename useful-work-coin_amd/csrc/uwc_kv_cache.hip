@@ -11,7 +11,7 @@
 //   read    value = z s of a range of tokens, rounded once to the output type; zeros in rows of no sequence.
 //
 // Bytes bound both where tokens are many (a prefill of 3890 tokens, 16 + 2 x 8 heads of 128: 60 MB in 15.8 us; 30000 tokens
-// read back, 184 MB in 36.0 us, 5.1 TB/s), the chain cu -> table -> rows -> scale where they are few (one token 4.0 us,
+// read back, 184 MB in 35.2 us, 5.2 TB/s), the chain cu -> table -> rows -> scale where they are few (one token 4.0 us,
 // 96 of them 6.3). A head row of hd dims is held by hd / 16 lanes, each with 8 dims of the lower half and
 // the 8 that rotate with them, so the rotation stays in a lane and loads are 16 bytes wide.
 #include "uwc_kv.h"
