@@ -466,6 +466,27 @@ int uwc_kv_read(const int8_t* k, const int8_t* v, const float* ks, const float* 
                 int hd, const int32_t* table, int64_t table_stride, int width, const int32_t* start, const int32_t* cu,
                 int B, int rows, int dtype, void* ko, void* vo, hipStream_t stream);
 
+/* ======================================================================== linears with 4-bit weights
+ * Weights in the OCP microscaling format of fp4 elements, rows in 16 bits (UWC_W4_BF16 or UWC_W4_FP16). No counterpart
+ * in the reference (its linears are 8-bit, runtime/detrt/qwen3.py:71-126).
+ *
+ * Row n of a weight: codes K / 2 bytes, the weight of the lower k in a byte's low half, and scales K / 32 bytes:
+ * w[n, k] = value(code) 2^(scale[n, k / 32] - 127), value = 0, 0.5, 1, 1.5, 2, 3, 4, 6, negated where the code's top
+ * bit is set; a scale of 255 makes its row's outputs NaN. Rows are dense, K a positive multiple of 32. x: M rows,
+ * x_stride elements apart; x, its rows and codes 16-byte aligned, y (dense, x's type) 8-byte aligned. Sums are fp32,
+ * rounded once; bf16 rows meet the weights exactly, fp16 rows the weights rounded to fp16 (exact for scales from 103 to 140). */
+#define UWC_W4_BF16 0
+#define UWC_W4_FP16 1
+
+/* y[m, n] = sum_k x[m, k] w[n, k] (+ bias[n], of x's type; NULL: none), n < N. */
+int uwc_w4_linear(const void* x, int64_t x_stride, int dtype, int M, const uint8_t* codes, const uint8_t* scales, int N,
+                  int K, const void* bias, void* y, hipStream_t stream);
+
+/* y[m, f] = silu(sum_k x[m, k] w[f, k]) sum_k x[m, k] w[F + f, k], f < F: a feed-forward block's gate and up projections
+ * (2 F rows of weights, the gate's first), the activation and the product. */
+int uwc_w4_gated(const void* x, int64_t x_stride, int dtype, int M, const uint8_t* codes, const uint8_t* scales, int F,
+                 int K, void* y, hipStream_t stream);
+
 /* Measurement aid (no reference counterpart): iters x 8 v_mfma_i32_32x32x32_i8 per wave in a
  * register-only loop, 8 waves on every CU, with constant (random_operands = 0) or seeded random
  * operands; each MFMA is 65,536 int8 ops. Timing it gives the part's sustained int8 MFMA rate,

@@ -1,0 +1,170 @@
+// Linears with 4-bit weights for few rows: the weights are streamed once per 16 to 64 rows, straight from memory into
+// the registers that the matrix instructions read.
+#include "uwc_w4.h"
+
+namespace {
+
+// A workgroup makes 16 NT weight rows times 16 MT rows of x (where GATED, 8 NT outputs: half of the NT tiles are gate
+// rows, half the matching up rows); its waves take every W-th block of 128 k and add up in LDS. In a block, lane
+// (i = lane % 16, j = lane / 16) holds weight row i's group j, 32 codes in 16 bytes with one scale, and x row i's same 32
+// values; step t multiplies elements 8 t .. 8 t + 7 of every group, so the k order inside a block differs from memory's, alike for both.
+template <class T, int MT, int NT, int W, bool GATED>
+__global__ __launch_bounds__(64 * W) void w4_rows_kernel(W4Args a, int nb, int mb) {
+  typedef typename W4<T>::v8 v8;
+  constexpr int OT = GATED ? NT / 2 : NT;  // tiles of outputs
+  __shared__ f4v red[W * MT * NT * 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // the workgroups of one weight block on one XCD: its L2 then reads the weights once
+  const int id = blockIdx.x, n_blk = id / (8 * mb) * 8 + id % 8, m_blk = id / 8 % mb;
+  if (n_blk >= nb) return;
+  const int i = lane & 15, j = lane >> 4, groups = a.K / 32, blocks = (groups + 3) / 4;
+  const int n0 = n_blk * 16 * OT, m0 = m_blk * 16 * MT;
+  const u8 *cp[NT], *sp[NT];
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    int n = n0 + 16 * (t % OT) + i;
+    n = (n < a.F ? n : a.F - 1) + (t >= OT ? a.F : 0);  // rows past the last are read twice and not stored
+    cp[t] = a.codes + (long)n * (a.K / 2);
+    sp[t] = a.scales + (long)n * groups;
+  }
+  const T* xp[MT];
+  bool there[MT];
+#pragma unroll
+  for (int t = 0; t < MT; t++) {
+    const int m = m0 + 16 * t + i;
+    there[t] = m < a.M;
+    xp[t] = static_cast<const T*>(a.x) + (long)(there[t] ? m : 0) * a.x_stride;
+  }
+  f4v acc[MT][NT];
+#pragma unroll
+  for (int p = 0; p < MT; p++)
+#pragma unroll
+    for (int t = 0; t < NT; t++) acc[p][t] = f4v{0, 0, 0, 0};
+
+  struct Weights {
+    w4_u4 c[NT];
+    float s[NT];
+  };
+  struct Rows {
+    v8 x[MT][4];
+  };
+  auto load = [&](Weights& p, int b) W4_AI {
+    const int g = 4 * b + j < groups ? 4 * b + j : groups - 1;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      p.c[t] = *reinterpret_cast<const w4_u4*>(cp[t] + g * 16);
+      p.s[t] = __uint_as_float((u32)sp[t][g] << 23);
+    }
+  };
+  auto load_rows = [&](Rows& p, int b) W4_AI {
+    const int g = 4 * b + j;
+#pragma unroll
+    for (int q = 0; q < MT; q++)
+#pragma unroll
+      for (int t = 0; t < 4; t++) {
+        v8 z = {};
+        if (there[q] && g < groups) z = *reinterpret_cast<const v8*>(xp[q] + g * 32 + t * 8);
+        p.x[q][t] = z;
+      }
+  };
+  auto mul = [&](const Weights& p, const Rows& r) W4_AI {
+#pragma unroll
+    for (int t = 0; t < 4; t++)
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        const v8 w = W4<T>::weights(p.c[n][t], p.s[n]);
+#pragma unroll
+        for (int q = 0; q < MT; q++) acc[q][n] = W4<T>::mul(w, r.x[q][t], acc[q][n]);
+      }
+  };
+  // the next block's weights, and for few rows its x, are on their way while this one is multiplied
+  int b = wave;
+  if (b < blocks) {
+    Weights now;
+    Rows x;
+    load(now, b);
+    load_rows(x, b);
+    for (; b + W < blocks; b += W) {
+      Weights next;
+      load(next, b + W);
+      if constexpr (MT == 1) {
+        Rows nx;
+        load_rows(nx, b + W);
+        mul(now, x);
+        x = nx;
+      } else {
+        mul(now, x);
+        load_rows(x, b + W);
+      }
+      now = next;
+    }
+    mul(now, x);
+  }
+  // lane (i, j) holds outputs 4 j .. 4 j + 3 of row i; sums over the waves in their order
+#pragma unroll
+  for (int q = 0; q < MT; q++)
+#pragma unroll
+    for (int t = 0; t < NT; t++) red[((wave * MT + q) * NT + t) * 64 + lane] = acc[q][t];
+  __syncthreads();
+  for (int e = threadIdx.x; e < MT * OT * 64; e += 64 * W) {
+    const int q = e / (OT * 64), t = e / 64 % OT, l = e % 64;
+    auto sum = [&](int t) W4_AI {
+      f4v v = red[(q * NT + t) * 64 + l];
+      for (int w = 1; w < W; w++) v += red[((w * MT + q) * NT + t) * 64 + l];
+      return v;
+    };
+    f4v v = sum(t);
+    if (GATED) {
+      const f4v u = sum(OT + t);
+#pragma unroll
+      for (int r = 0; r < 4; r++) v[r] = w4_silu(v[r]) * u[r];
+    }
+    const int m = m0 + 16 * q + (l & 15), n = n0 + 16 * t + 4 * (l >> 4);
+    if (m < a.M && n < a.F) w4_store<T>(a, m, n, v);
+  }
+}
+
+template <class T, int MT, int NT, int W, bool GATED>
+int rows(const char* fn, const W4Args& a, hipStream_t stream) {
+  constexpr int out = 16 * (GATED ? NT / 2 : NT);
+  const long nb = ((long)a.F + out - 1) / out, mb = ((long)a.M + 16 * MT - 1) / (16 * MT);
+  const long blocks = (nb + 7) / 8 * 8 * mb;
+  if (blocks > 0xFFFFFFFFL / (64 * W)) return uwc_fail("%s: too many rows (%d) and outputs (%d)", fn, a.M, a.F);
+  hipLaunchKernelGGL((w4_rows_kernel<T, MT, NT, W, GATED>), dim3((unsigned)blocks), dim3(64 * W), 0, stream, a, (int)nb, (int)mb);
+  return uwc_launch_status(fn);
+}
+
+template <class T>
+int run(const char* fn, const W4Args& a, bool gated, hipStream_t stream) {
+  if (gated) {
+    if (a.M <= 16) return rows<T, 1, 2, 8, true>(fn, a, stream);
+    if (a.M <= 32) return rows<T, 2, 2, 8, true>(fn, a, stream);
+    return rows<T, 4, 2, 4, true>(fn, a, stream);
+  }
+  if (a.M <= 16) return rows<T, 1, 1, 8, false>(fn, a, stream);
+  if (a.M <= 32) return rows<T, 2, 1, 8, false>(fn, a, stream);
+  return rows<T, 4, 2, 4, false>(fn, a, stream);
+}
+
+int call(const char* fn, const W4Args& a, int dtype, bool gated, hipStream_t stream) {
+  if (dtype != UWC_W4_BF16 && dtype != UWC_W4_FP16) return uwc_fail("%s: unknown dtype %d", fn, dtype);
+  if (a.M < 0 || a.F < 0 || (gated && a.F > 0x3fffffff)) return uwc_fail("%s: bad M=%d N=%d", fn, a.M, a.F);
+  if (a.K <= 0 || a.K % 32) return uwc_fail("%s: K=%d must be a positive multiple of 32", fn, a.K);
+  if (a.M == 0 || a.F == 0) return UWC_OK;
+  if (!a.x || !a.codes || !a.scales || !a.y) return uwc_fail("%s: null arguments", fn);
+  if (a.x_stride < 0 || a.x_stride % 8 || (((uintptr_t)a.x | (uintptr_t)a.codes) & 15) || ((uintptr_t)a.y & 7))
+    return uwc_fail("%s: rows of x and codes must be 16-byte aligned, y 8-byte aligned", fn);
+  return dtype == UWC_W4_BF16 ? run<__bf16>(fn, a, gated, stream) : run<_Float16>(fn, a, gated, stream);
+}
+
+}  // namespace
+
+extern "C" int uwc_w4_linear(const void* x, int64_t x_stride, int dtype, int M, const uint8_t* codes, const uint8_t* scales,
+                             int N, int K, const void* bias, void* y, hipStream_t stream) {
+  return call("uwc_w4_linear", W4Args{x, (long)x_stride, codes, scales, bias, y, M, N, N, K}, dtype, false, stream);
+}
+
+extern "C" int uwc_w4_gated(const void* x, int64_t x_stride, int dtype, int M, const uint8_t* codes, const uint8_t* scales,
+                            int F, int K, void* y, hipStream_t stream) {
+  return call("uwc_w4_gated", W4Args{x, (long)x_stride, codes, scales, nullptr, y, M, F, F > 0x3fffffff ? F : 2 * F, K}, dtype, true, stream);
+}

@@ -77,6 +77,8 @@ SIGNATURES = {
     "uwc_kv_attend": [vp, vp, vp, vp, i64, i32, i32, i32, vp, i64, i32, i32, i32, vp, i64, i32, vp, vp, i32, i32, i32, i32, i32,
                       f32, vp, u64, vp, vp],
     "uwc_kv_read": [vp, vp, vp, vp, i64, i32, i32, i32, vp, i64, i32, vp, vp, i32, i32, i32, vp, vp, vp],
+    "uwc_w4_linear": [vp, i64, i32, i32, vp, vp, i32, i32, vp, vp, vp],
+    "uwc_w4_gated": [vp, i64, i32, i32, vp, vp, i32, i32, vp, vp],
     "uwc_mfma_rate_probe": [i32, i32, vp, i64, vp],
 }
 _RESTYPE = {"uwc_last_error": ctypes.c_char_p, "uwc_header_sha": ctypes.c_char_p,
