@@ -57,17 +57,24 @@ struct W4Args {
 
 __device__ __forceinline__ float w4_silu(float g) { return g / (1.0f + __expf(-g)); }
 
-// Four outputs n .. n + 3 of row m; four at once where rows of y stay aligned to that.
+// v + bias for outputs n .. n + 3
 template <class T>
-__device__ __forceinline__ void w4_store(const W4Args& a, int m, int n, f4v v) {
-  typedef T v4 __attribute__((ext_vector_type(4)));
-  T* y = static_cast<T*>(a.y) + (long)m * a.F + n;
+__device__ __forceinline__ f4v w4_bias(const W4Args& a, int n, f4v v) {
   if (a.bias) {
     const T* b = static_cast<const T*>(a.bias);
 #pragma unroll
     for (int r = 0; r < 4; r++) v[r] += (float)b[n + r < a.F ? n + r : a.F - 1];
   }
-  if (a.F % 4 == 0 && n + 3 < a.F) {
+  return v;
+}
+
+// Four outputs n .. n + 3 of row m; four at once where rows of y stay aligned to that.
+template <class T>
+__device__ __forceinline__ void w4_store(const W4Args& a, int m, int n, f4v v) {
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  T* y = static_cast<T*>(a.y) + (long)m * a.F + n;
+  v = w4_bias<T>(a, n, v);
+  if (a.F % 4 == 0) {
     v4 o = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
     *reinterpret_cast<v4*>(y) = o;
   } else {

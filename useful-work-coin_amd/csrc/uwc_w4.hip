@@ -149,11 +149,13 @@ int run(const char* fn, const W4Args& a, bool gated, hipStream_t stream) {
 int call(const char* fn, const W4Args& a, int dtype, bool gated, hipStream_t stream) {
   if (dtype != UWC_W4_BF16 && dtype != UWC_W4_FP16) return uwc_fail("%s: unknown dtype %d", fn, dtype);
   if (a.M < 0 || a.F < 0 || (gated && a.F > 0x3fffffff)) return uwc_fail("%s: bad M=%d N=%d", fn, a.M, a.F);
-  if (a.K <= 0 || a.K % 32) return uwc_fail("%s: K=%d must be a positive multiple of 32", fn, a.K);
+  if (a.K <= 0 || a.K % 32 || a.K > 1 << 22) return uwc_fail("%s: K=%d must be a positive multiple of 32, at most 2^22", fn, a.K);
   if (a.M == 0 || a.F == 0) return UWC_OK;
   if (!a.x || !a.codes || !a.scales || !a.y) return uwc_fail("%s: null arguments", fn);
+  if (a.x_stride > 1 << 22) return uwc_fail("%s: rows of x are %ld elements apart, more than 2^22", fn, a.x_stride);
   if (a.x_stride < 0 || a.x_stride % 8 || (((uintptr_t)a.x | (uintptr_t)a.codes) & 15) || ((uintptr_t)a.y & 7))
     return uwc_fail("%s: rows of x and codes must be 16-byte aligned, y 8-byte aligned", fn);
+  if (w4_gemm_pays(a.M, a.F, a.K, gated)) return w4_gemm(fn, a, dtype, gated, stream);
   return dtype == UWC_W4_BF16 ? run<__bf16>(fn, a, gated, stream) : run<_Float16>(fn, a, gated, stream);
 }
 

@@ -1,0 +1,213 @@
+// Linears with 4-bit weights for many rows: x in LDS tiles, the weights straight from memory into the registers that
+// the matrix instructions read.
+#include "uwc_w4.h"
+
+namespace {
+
+// A workgroup of WM x WN waves makes 64 WM rows of x times 32 NT WN weight rows (where GATED half of a wave's tiles are gate
+// rows and the other half the matching up rows), a wave 64 x 32 NT of them on 32 x 32 x 16 instructions. A step is 64 k, two
+// groups: lane (i = lane % 32, h = lane / 32) holds weight row i's group h, 32 codes in 16 bytes with one scale, and x's
+// values of that group; instruction t multiplies elements 8 t .. 8 t + 7 of both groups.
+// Both operands come through LDS, read from memory in whole lines: x by steps, the codes and scales by four steps (128 bytes of a
+// row), a quarter of the rows in each step. Each has two buffers. LDS rows are 128 bytes, their 16-byte chunk c at
+// c ^ (row / 2 % 8): sixteen lanes that read one chunk of successive rows then touch all 64 banks. Codes straight from
+// memory, 32 bytes of each row at a time and by every wave that needs them, kept the address units busier than the matrix units.
+template <class T, int WM, int WN, int NT, bool GATED>
+__global__ __launch_bounds__(64 * WM * WN) void w4_gemm_kernel(W4Args a, int mb, int nb) {
+  typedef typename W4<T>::v8 v8;
+  constexpr int WAVES = WM * WN, BM = 64 * WM, THREADS = 64 * WAVES, OT = GATED ? NT / 2 : NT, BN = 32 * OT * WN;
+  constexpr int ROWS = 32 * NT * WN;  // of weights
+  constexpr int CHUNKS = BM * 8 / THREADS, PIECE = ROWS * 8 / 4 / THREADS;
+  static_assert(PIECE == 1 && ROWS * 2 == THREADS, "a thread stages 16 bytes of codes and one scale a step");
+  __shared__ __attribute__((aligned(16))) u8 lds[2][BM * 128];
+  __shared__ __attribute__((aligned(16))) u8 codes_lds[2][ROWS * 128];
+  __shared__ __attribute__((aligned(16))) u8 scales_lds[2][ROWS * 8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN, i = lane & 31, h = lane >> 5;
+  // an XCD takes neighbouring tiles, eight of x's to one of the weight's: its L2 holds what they share
+  const int per = (mb * nb + 7) / 8;
+  const int tile = blockIdx.x % 8 * per + blockIdx.x / 8;
+  if (tile >= mb * nb) return;
+  const int band = tile / (8 * nb), rows_in = mb - 8 * band < 8 ? mb - 8 * band : 8, in = tile - band * 8 * nb;
+  const int m0 = (8 * band + in % rows_in) * BM, n0 = in / rows_in * BN;
+  const int groups = a.K / 32, steps = (groups + 1) / 2;
+
+  // row r of the workgroup's weight rows: tile r / 32, of wave column r / (32 NT); rows past the last are the last, and not stored
+  auto weight_row = [&](int r) W4_AI {
+    const int t = r / 32 % NT, n = n0 + (r / (32 * NT) * OT + t % OT) * 32 + r % 32;
+    return (long)(n < a.F ? n : a.F - 1) + (t >= OT ? a.F : 0);
+  };
+  const u8* x_at = static_cast<const u8*>(a.x) + (long)m0 * a.x_stride * 2;
+  u32 x_off[CHUNKS], to[CHUNKS], from[2], code_from[NT];
+  const int chunk = tid & 7;
+#pragma unroll
+  for (int c = 0; c < CHUNKS; c++) {
+    const int r = (tid >> 3) + c * (THREADS / 8), m = m0 + r < a.M ? r : a.M - 1 - m0;
+    x_off[c] = (u32)m * (u32)a.x_stride * 2;
+    to[c] = r * 128 + ((chunk ^ (r >> 1)) & 7) * 16;
+  }
+#pragma unroll
+  for (int q = 0; q < 2; q++) {  // x rows i and 32 + i of this wave, chunk 4 h
+    const int r = wm * 64 + 32 * q + i;
+    from[q] = r * 128 + (((4 * h) ^ (r >> 1)) & 7) * 16;
+  }
+#pragma unroll
+  for (int t = 0; t < NT; t++) {  // weight row i of each tile, chunk h
+    const int r = (wn * NT + t) * 32 + i;
+    code_from[t] = r * 128 + ((h ^ (r >> 1)) & 7) * 16;
+  }
+  // this thread's weight rows: of piece j of the codes, and of the scales
+  const u8* code_at[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) code_at[j] = a.codes + weight_row(j * (ROWS / 4) + (tid >> 3)) * (a.K / 2);
+  const u8* scale_at = a.scales + weight_row(tid >> 1) * groups;
+
+  w4_u4 xr[CHUNKS], piece;
+  u32 scale_byte;
+  auto load_x = [&](int s) W4_AI {  // a step's second group may not be there: the first again
+    const u32 at = 2 * s + 1 < groups ? chunk * 16 : (chunk & 3) * 16;
+#pragma unroll
+    for (int c = 0; c < CHUNKS; c++) xr[c] = *reinterpret_cast<const w4_u4*>(x_at + (long)s * 128 + (x_off[c] + at));
+  };
+  auto put_x = [&](int s) W4_AI {
+    if (2 * s + 1 >= groups && chunk >= 4) {
+#pragma unroll
+      for (int c = 0; c < CHUNKS; c++) xr[c] = w4_u4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int c = 0; c < CHUNKS; c++) *reinterpret_cast<w4_u4*>(&lds[s & 1][to[c]]) = xr[c];
+  };
+  // piece 4 S + j: of the eight groups of steps 4 S .. 4 S + 3 the codes of a quarter of the rows, and bytes j and 4 + j of every
+  // row's scales; groups past the last are the last, and meet zeros of x
+  auto load_piece = [&](int S, int j) W4_AI {
+    const int g = 8 * S + chunk, e = 8 * S + 4 * (tid & 1) + j;
+    piece = *reinterpret_cast<const w4_u4*>(code_at[j] + (g < groups ? g : groups - 1) * 16);
+    scale_byte = scale_at[e < groups ? e : groups - 1];
+  };
+  auto put_piece = [&](int S, int j) W4_AI {
+    const int r = j * (ROWS / 4) + (tid >> 3);
+    *reinterpret_cast<w4_u4*>(&codes_lds[S & 1][r * 128 + ((chunk ^ (r >> 1)) & 7) * 16]) = piece;
+    scales_lds[S & 1][(tid >> 1) * 8 + 4 * (tid & 1) + j] = (u8)scale_byte;
+  };
+  w4_f16 acc[2][NT];
+#pragma unroll
+  for (int q = 0; q < 2; q++)
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) acc[q][t][r] = 0;
+
+  // Loads never depend on a branch, so that the compiler waits for those it needs and no more: the last steps load the
+  // last one again.
+  load_x(0);
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    load_piece(0, j);
+    put_piece(0, j);
+  }
+  load_piece(1, 0);
+  put_x(0);
+  load_x(steps > 1 ? 1 : 0);
+  __syncthreads();
+  for (int S = 0; 4 * S < steps; S++) {
+    u2v scale[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      scale[t] = *reinterpret_cast<const u2v*>(&scales_lds[S & 1][((wn * NT + t) * 32 + i) * 8]);
+      scale[t][0] >>= 8 * h, scale[t][1] >>= 8 * h;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int s = 4 * S + j;
+      if (s >= steps) break;
+      const u8* buf = lds[s & 1];
+      v8 x[2][2];
+      w4_u4 codes[NT];
+#pragma unroll
+      for (int q = 0; q < 2; q++) x[0][q] = *reinterpret_cast<const v8*>(buf + from[q]);
+#pragma unroll
+      for (int t = 0; t < NT; t++) codes[t] = *reinterpret_cast<const w4_u4*>(&codes_lds[S & 1][code_from[t] ^ (j * 32)]);
+      // what the next step, or the next four, will read has had a whole step to arrive; its place was last read before a barrier
+      put_x(s + 1);
+      put_piece(S + 1, j);
+      load_x(s + 2 < steps ? s + 2 : steps - 1);
+      load_piece(j < 3 ? S + 1 : S + 2, (j + 1) & 3);
+      __builtin_amdgcn_sched_barrier(0);  // on their way now, not where the registers are short
+#pragma unroll
+      for (int t = 0; t < 4; t++) {
+        if (t < 3) {
+#pragma unroll
+          for (int q = 0; q < 2; q++) x[(t + 1) & 1][q] = *reinterpret_cast<const v8*>(buf + (from[q] ^ ((t + 1) * 16)));
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          const u32 f = (scale[n][j >> 1] >> (16 * (j & 1)) & 0xff) << 23;
+          const v8 w = W4<T>::weights(codes[n][t], __uint_as_float(f));
+#pragma unroll
+          for (int q = 0; q < 2; q++) acc[q][n] = W4<T>::mul32(w, x[t & 1][q], acc[q][n]);
+        }
+      }
+      __syncthreads();
+    }
+  }
+  auto value = [&](int q, int t, int r) W4_AI {
+    f4v v = {acc[q][t][4 * r], acc[q][t][4 * r + 1], acc[q][t][4 * r + 2], acc[q][t][4 * r + 3]};
+    if (GATED) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = w4_silu(v[e]) * acc[q][(OT + t) % NT][4 * r + e];
+    }
+    return v;
+  };
+  const int mw = m0 + wm * 64, nw = n0 + wn * OT * 32;
+  if (a.F % 8 || ((uintptr_t)a.y & 15)) {
+#pragma unroll
+    for (int q = 0; q < 2; q++)
+#pragma unroll
+      for (int t = 0; t < OT; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int m = mw + 32 * q + i, n = nw + 32 * t + 8 * r + 4 * h;
+          if (m < a.M && n < a.F) w4_store<T>(a, m, n, value(q, t, r));
+        }
+    return;
+  }
+  // 32 rows of this wave's outputs at a time through its own part of LDS, so that a row's bytes leave together
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  constexpr int ROW = 64 * OT, PER = ROW / 16;  // bytes, 16-byte chunks of a row
+  static_assert(WAVES * 32 * ROW <= (int)sizeof lds, "the waves' parts fit");
+  u8* part = &lds[0][0] + wave * 32 * ROW;
+#pragma unroll
+  for (int q = 0; q < 2; q++) {
+#pragma unroll
+    for (int t = 0; t < OT; t++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const f4v v = w4_bias<T>(a, nw + 32 * t + 8 * r + 4 * h, value(q, t, r));
+        *reinterpret_cast<v4*>(part + i * ROW + (((4 * t + r) ^ i) % PER) * 16 + 8 * h) = v4{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+      }
+#pragma unroll
+    for (int e = 0; e < 32 * PER / 64; e++) {
+      const int row = (e * 64 + lane) / PER, c = lane % PER, m = mw + 32 * q + row, n = nw + 8 * c;
+      const w4_u4 z = *reinterpret_cast<const w4_u4*>(part + row * ROW + ((c ^ row) % PER) * 16);
+      if (m < a.M && n < a.F) *reinterpret_cast<w4_u4*>(static_cast<T*>(a.y) + (long)m * a.F + n) = z;
+    }
+  }
+}
+
+template <class T, int WM, int WN, int NT, bool GATED>
+int launch(const char* fn, const W4Args& a, hipStream_t stream) {
+  constexpr int BM = 64 * WM, BN = 32 * (GATED ? NT / 2 : NT) * WN;
+  const long mb = ((long)a.M + BM - 1) / BM, nb = ((long)a.F + BN - 1) / BN, blocks = (mb * nb + 7) / 8 * 8;
+  if (blocks > 0x7fffffffL / (64 * WM * WN)) return uwc_fail("%s: too many rows (%d) and outputs (%d)", fn, a.M, a.F);
+  hipLaunchKernelGGL((w4_gemm_kernel<T, WM, WN, NT, GATED>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a, (int)mb, (int)nb);
+  return uwc_launch_status(fn);
+}
+
+}  // namespace
+
+bool w4_gemm_pays(int M, int F, int K, bool gated) { return M > 128; }
+
+int w4_gemm(const char* fn, const W4Args& a, int dtype, bool gated, hipStream_t stream) {
+  if (dtype == UWC_W4_BF16) return gated ? launch<__bf16, 4, 2, 4, true>(fn, a, stream) : launch<__bf16, 4, 2, 4, false>(fn, a, stream);
+  return gated ? launch<_Float16, 4, 2, 4, true>(fn, a, stream) : launch<_Float16, 4, 2, 4, false>(fn, a, stream);
+}

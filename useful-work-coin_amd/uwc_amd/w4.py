@@ -98,7 +98,7 @@ def _call(fn, x, codes, scales):
     if x.device.type != "cuda":
         raise AssertionError(f"{fn}: the weight must be on a GPU, got {x.device}")
     rows = x.reshape(-1, K)
-    if not (rows.stride(1) == 1 and rows.stride(0) % 8 == 0 and rows.stride(0) >= 0 and rows.data_ptr() % 16 == 0):
+    if not (rows.stride(1) == 1 and rows.stride(0) % 8 == 0 and 0 <= rows.stride(0) <= 1 << 22 and rows.data_ptr() % 16 == 0):
         rows = rows.clone(memory_format=torch.contiguous_format)
     return rows, N, K
 
