@@ -84,6 +84,5 @@ __device__ __forceinline__ void w4_store(const W4Args& a, int m, int n, f4v v) {
   }
 }
 
-// The kernel for many rows (uwc_w4_gemm.hip); false where it does not pay.
-bool w4_gemm_pays(int M, int F, int K, bool gated);
+// The kernel for many rows (uwc_w4_gemm.hip).
 int w4_gemm(const char* fn, const W4Args& a, int dtype, bool gated, hipStream_t stream);

@@ -5,9 +5,10 @@
 namespace {
 
 // A workgroup makes 16 NT weight rows times 16 MT rows of x (where GATED, 8 NT outputs: half of the NT tiles are gate
-// rows, half the matching up rows); its waves take every W-th block of 128 k and add up in LDS. In a block, lane
-// (i = lane % 16, j = lane / 16) holds weight row i's group j, 32 codes in 16 bytes with one scale, and x row i's same 32
-// values; step t multiplies elements 8 t .. 8 t + 7 of every group, so the k order inside a block differs from memory's, alike for both.
+// rows, half the matching up rows); its waves take every W-th unit of 256 k and add up in LDS. In a unit, lane
+// (i = lane % 16, j = lane / 16) holds weight row i's groups 2 j and 2 j + 1, 64 codes in 32 bytes with two scales, and x row i's
+// same 64 values; step t multiplies elements 8 t .. 8 t + 7 of the first groups, step 4 + t of the second, so the k order inside
+// a unit differs from memory's, alike for both. Whole lines of 128 bytes of codes are read, and all of a wave's first two units at once.
 template <class T, int MT, int NT, int W, bool GATED>
 __global__ __launch_bounds__(64 * W) void w4_rows_kernel(W4Args a, int nb, int mb) {
   typedef typename W4<T>::v8 v8;
@@ -17,7 +18,7 @@ __global__ __launch_bounds__(64 * W) void w4_rows_kernel(W4Args a, int nb, int m
   // the workgroups of one weight block on one XCD: its L2 then reads the weights once
   const int id = blockIdx.x, n_blk = id / (8 * mb) * 8 + id % 8, m_blk = id / 8 % mb;
   if (n_blk >= nb) return;
-  const int i = lane & 15, j = lane >> 4, groups = a.K / 32, blocks = (groups + 3) / 4;
+  const int i = lane & 15, j = lane >> 4, groups = a.K / 32, units = (groups + 7) / 8;
   const int n0 = n_blk * 16 * OT, m0 = m_blk * 16 * MT;
   const u8 *cp[NT], *sp[NT];
 #pragma unroll
@@ -42,59 +43,68 @@ __global__ __launch_bounds__(64 * W) void w4_rows_kernel(W4Args a, int nb, int m
     for (int t = 0; t < NT; t++) acc[p][t] = f4v{0, 0, 0, 0};
 
   struct Weights {
-    w4_u4 c[NT];
-    float s[NT];
+    w4_u4 c[NT][2];
+    u32 s[NT];
   };
   struct Rows {
-    v8 x[MT][4];
+    v8 x[MT][8];
   };
-  auto load = [&](Weights& p, int b) W4_AI {
-    const int g = 4 * b + j < groups ? 4 * b + j : groups - 1;
+  auto load = [&](Weights& p, int u) W4_AI {
+    // groups that are not there are others of the row, which meet zeros of x
+    const int g = 8 * u + 2 * j, g0 = g < groups ? g : groups - 1, g1 = g + 1 < groups ? g + 1 : groups - 1;
+    const int pair = g0 < groups - 1 ? g0 : groups - 2;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      p.c[t] = *reinterpret_cast<const w4_u4*>(cp[t] + g * 16);
-      p.s[t] = __uint_as_float((u32)sp[t][g] << 23);
+      p.c[t][0] = *reinterpret_cast<const w4_u4*>(cp[t] + g0 * 16);
+      p.c[t][1] = *reinterpret_cast<const w4_u4*>(cp[t] + g1 * 16);
+      if (groups > 1) {
+        unsigned short two;  // at any address: rows may hold an odd number of scales
+        __builtin_memcpy(&two, sp[t] + pair, 2);
+        p.s[t] = (u32)two >> (8 * (g0 - pair));
+      } else {
+        p.s[t] = *sp[t];
+      }
     }
   };
-  auto load_rows = [&](Rows& p, int b) W4_AI {
-    const int g = 4 * b + j;
+  auto load_rows = [&](Rows& p, int u) W4_AI {
+    const int g = 8 * u + 2 * j;
 #pragma unroll
     for (int q = 0; q < MT; q++)
 #pragma unroll
-      for (int t = 0; t < 4; t++) {
+      for (int t = 0; t < 8; t++) {
         v8 z = {};
-        if (there[q] && g < groups) z = *reinterpret_cast<const v8*>(xp[q] + g * 32 + t * 8);
+        if (there[q] && g + t / 4 < groups) z = *reinterpret_cast<const v8*>(xp[q] + g * 32 + t * 8);
         p.x[q][t] = z;
       }
   };
   auto mul = [&](const Weights& p, const Rows& r) W4_AI {
 #pragma unroll
-    for (int t = 0; t < 4; t++)
+    for (int t = 0; t < 8; t++)
 #pragma unroll
       for (int n = 0; n < NT; n++) {
-        const v8 w = W4<T>::weights(p.c[n][t], p.s[n]);
+        const v8 w = W4<T>::weights(p.c[n][t / 4][t % 4], __uint_as_float((p.s[n] >> (t / 4 * 8) & 0xff) << 23));
 #pragma unroll
         for (int q = 0; q < MT; q++) acc[q][n] = W4<T>::mul(w, r.x[q][t], acc[q][n]);
       }
   };
-  // the next block's weights, and for few rows its x, are on their way while this one is multiplied
-  int b = wave;
-  if (b < blocks) {
+  // the next unit's weights, and for few rows its x, are on their way while this one is multiplied
+  int u = wave;
+  if (u < units) {
     Weights now;
     Rows x;
-    load(now, b);
-    load_rows(x, b);
-    for (; b + W < blocks; b += W) {
+    load(now, u);
+    load_rows(x, u);
+    for (; u + W < units; u += W) {
       Weights next;
-      load(next, b + W);
+      load(next, u + W);
       if constexpr (MT == 1) {
         Rows nx;
-        load_rows(nx, b + W);
+        load_rows(nx, u + W);
         mul(now, x);
         x = nx;
       } else {
         mul(now, x);
-        load_rows(x, b + W);
+        load_rows(x, u + W);
       }
       now = next;
     }
@@ -134,16 +144,14 @@ int rows(const char* fn, const W4Args& a, hipStream_t stream) {
   return uwc_launch_status(fn);
 }
 
+// More tiles of weights to a workgroup share the loads of x, fewer keep all compute units at work.
 template <class T>
 int run(const char* fn, const W4Args& a, bool gated, hipStream_t stream) {
-  if (gated) {
-    if (a.M <= 16) return rows<T, 1, 2, 8, true>(fn, a, stream);
-    if (a.M <= 32) return rows<T, 2, 2, 8, true>(fn, a, stream);
-    return rows<T, 4, 2, 4, true>(fn, a, stream);
-  }
-  if (a.M <= 16) return rows<T, 1, 1, 8, false>(fn, a, stream);
-  if (a.M <= 32) return rows<T, 2, 1, 8, false>(fn, a, stream);
-  return rows<T, 4, 2, 4, false>(fn, a, stream);
+  if (gated) return a.F >= 8192 || a.M > 4 ? rows<T, 1, 4, 4, true>(fn, a, stream) : rows<T, 1, 2, 4, true>(fn, a, stream);
+  if (a.M > 16) return rows<T, 2, 1, 8, false>(fn, a, stream);
+  if (a.F >= 16384) return rows<T, 1, 2, 4, false>(fn, a, stream);
+  if (a.F >= 6144) return rows<T, 1, 2, 8, false>(fn, a, stream);
+  return rows<T, 1, 1, 8, false>(fn, a, stream);
 }
 
 int call(const char* fn, const W4Args& a, int dtype, bool gated, hipStream_t stream) {
@@ -155,7 +163,7 @@ int call(const char* fn, const W4Args& a, int dtype, bool gated, hipStream_t str
   if (a.x_stride > 1 << 22) return uwc_fail("%s: rows of x are %ld elements apart, more than 2^22", fn, a.x_stride);
   if (a.x_stride < 0 || a.x_stride % 8 || (((uintptr_t)a.x | (uintptr_t)a.codes) & 15) || ((uintptr_t)a.y & 7))
     return uwc_fail("%s: rows of x and codes must be 16-byte aligned, y 8-byte aligned", fn);
-  if (w4_gemm_pays(a.M, a.F, a.K, gated)) return w4_gemm(fn, a, dtype, gated, stream);
+  if (a.M > (gated || a.F > 8192 ? 16 : 32)) return w4_gemm(fn, a, dtype, gated, stream);
   return dtype == UWC_W4_BF16 ? run<__bf16>(fn, a, gated, stream) : run<_Float16>(fn, a, gated, stream);
 }
 

@@ -12,17 +12,26 @@ namespace {
 // row), a quarter of the rows in each step. Each has two buffers. LDS rows are 128 bytes, their 16-byte chunk c at
 // c ^ (row / 2 % 8): sixteen lanes that read one chunk of successive rows then touch all 64 banks. Codes straight from
 // memory, 32 bytes of each row at a time and by every wave that needs them, kept the address units busier than the matrix units.
-template <class T, int WM, int WN, int NT, bool GATED>
-__global__ __launch_bounds__(64 * WM * WN) void w4_gemm_kernel(W4Args a, int mb, int nb) {
+// Where tiles of 256 x 256 leave compute units idle, smaller ones, and KG groups of waves that take every KG-th four steps of
+// the sums, each with its own buffers; they are added up through LDS, in the groups' order.
+template <class T, int KG, int WM, int WN, int NT, bool GATED>
+__global__ __launch_bounds__(64 * KG * WM * WN) void w4_gemm_kernel(W4Args a, int mb, int nb) {
   typedef typename W4<T>::v8 v8;
-  constexpr int WAVES = WM * WN, BM = 64 * WM, THREADS = 64 * WAVES, OT = GATED ? NT / 2 : NT, BN = 32 * OT * WN;
-  constexpr int ROWS = 32 * NT * WN;  // of weights
+  constexpr int WAVES = WM * WN, BM = 64 * WM, THREADS = 64 * WAVES;  // of a group
+  constexpr int ROWS = 32 * NT * WN, BN = GATED ? ROWS / 2 : ROWS;   // of weights, outputs
+  // the matching gate and up rows: tiles of one wave, or (one tile a wave) the first and second half of the waves
+  constexpr bool PAIRED = GATED && NT > 1;
+  constexpr int OT = PAIRED ? NT / 2 : NT;
   constexpr int CHUNKS = BM * 8 / THREADS, PIECE = ROWS * 8 / 4 / THREADS;
   static_assert(PIECE == 1 && ROWS * 2 == THREADS, "a thread stages 16 bytes of codes and one scale a step");
-  __shared__ __attribute__((aligned(16))) u8 lds[2][BM * 128];
-  __shared__ __attribute__((aligned(16))) u8 codes_lds[2][ROWS * 128];
-  __shared__ __attribute__((aligned(16))) u8 scales_lds[2][ROWS * 8];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN, i = lane & 31, h = lane >> 5;
+  struct Buffers {
+    u8 x[2][BM * 128], codes[2][ROWS * 128], scales[2][ROWS * 8];
+  };
+  constexpr int SUMS = KG > 1 ? KG * WAVES * NT * 8192 : 0;
+  __shared__ __attribute__((aligned(16))) u8 shared[sizeof(Buffers) * KG > SUMS ? sizeof(Buffers) * KG : SUMS];
+  const int kg = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS) : 0, tid = threadIdx.x % THREADS;
+  Buffers& L = reinterpret_cast<Buffers*>(shared)[kg];
+  const int lane = tid & 63, wave = tid >> 6, wm = wave / WN, wn = wave % WN, i = lane & 31, h = lane >> 5;
   // an XCD takes neighbouring tiles, eight of x's to one of the weight's: its L2 holds what they share
   const int per = (mb * nb + 7) / 8;
   const int tile = blockIdx.x % 8 * per + blockIdx.x / 8;
@@ -33,8 +42,10 @@ __global__ __launch_bounds__(64 * WM * WN) void w4_gemm_kernel(W4Args a, int mb,
 
   // row r of the workgroup's weight rows: tile r / 32, of wave column r / (32 NT); rows past the last are the last, and not stored
   auto weight_row = [&](int r) W4_AI {
-    const int t = r / 32 % NT, n = n0 + (r / (32 * NT) * OT + t % OT) * 32 + r % 32;
-    return (long)(n < a.F ? n : a.F - 1) + (t >= OT ? a.F : 0);
+    const int t = r / 32 % NT;
+    const bool up = PAIRED ? t >= OT : GATED && r >= BN;
+    const int n = n0 + (PAIRED ? (r / (32 * NT) * OT + t % OT) * 32 + r % 32 : GATED ? r % BN : r);
+    return (long)(n < a.F ? n : a.F - 1) + (up ? a.F : 0);
   };
   const u8* x_at = static_cast<const u8*>(a.x) + (long)m0 * a.x_stride * 2;
   u32 x_off[CHUNKS], to[CHUNKS], from[2], code_from[NT];
@@ -63,30 +74,31 @@ __global__ __launch_bounds__(64 * WM * WN) void w4_gemm_kernel(W4Args a, int mb,
 
   w4_u4 xr[CHUNKS], piece;
   u32 scale_byte;
-  auto load_x = [&](int s) W4_AI {  // a step's second group may not be there: the first again
+  auto load_x = [&](int s) W4_AI {  // steps past the last are the last; a step's second group may not be there: the first again
+    s = s < steps ? s : steps - 1;
     const u32 at = 2 * s + 1 < groups ? chunk * 16 : (chunk & 3) * 16;
 #pragma unroll
     for (int c = 0; c < CHUNKS; c++) xr[c] = *reinterpret_cast<const w4_u4*>(x_at + (long)s * 128 + (x_off[c] + at));
   };
   auto put_x = [&](int s) W4_AI {
-    if (2 * s + 1 >= groups && chunk >= 4) {
+    if (2 * s + 1 >= groups && (chunk >= 4 || 2 * s >= groups)) {
 #pragma unroll
       for (int c = 0; c < CHUNKS; c++) xr[c] = w4_u4{0, 0, 0, 0};
     }
 #pragma unroll
-    for (int c = 0; c < CHUNKS; c++) *reinterpret_cast<w4_u4*>(&lds[s & 1][to[c]]) = xr[c];
+    for (int c = 0; c < CHUNKS; c++) *reinterpret_cast<w4_u4*>(&L.x[s & 1][to[c]]) = xr[c];
   };
-  // piece 4 S + j: of the eight groups of steps 4 S .. 4 S + 3 the codes of a quarter of the rows, and bytes j and 4 + j of every
-  // row's scales; groups past the last are the last, and meet zeros of x
-  auto load_piece = [&](int S, int j) W4_AI {
-    const int g = 8 * S + chunk, e = 8 * S + 4 * (tid & 1) + j;
+  // piece j of four steps: of their eight groups, from `first` on, the codes of the j-th quarter of the rows, and bytes j and 4 + j of
+  // every row's scales; groups past the last are the last, and meet zeros of x
+  auto load_piece = [&](int first, int j) W4_AI {
+    const int g = first + chunk, e = first + 4 * (tid & 1) + j;
     piece = *reinterpret_cast<const w4_u4*>(code_at[j] + (g < groups ? g : groups - 1) * 16);
     scale_byte = scale_at[e < groups ? e : groups - 1];
   };
-  auto put_piece = [&](int S, int j) W4_AI {
+  auto put_piece = [&](int buf, int j) W4_AI {
     const int r = j * (ROWS / 4) + (tid >> 3);
-    *reinterpret_cast<w4_u4*>(&codes_lds[S & 1][r * 128 + ((chunk ^ (r >> 1)) & 7) * 16]) = piece;
-    scales_lds[S & 1][(tid >> 1) * 8 + 4 * (tid & 1) + j] = (u8)scale_byte;
+    *reinterpret_cast<w4_u4*>(&L.codes[buf][r * 128 + ((chunk ^ (r >> 1)) & 7) * 16]) = piece;
+    L.scales[buf][(tid >> 1) * 8 + 4 * (tid & 1) + j] = (u8)scale_byte;
   };
   w4_f16 acc[2][NT];
 #pragma unroll
@@ -98,39 +110,39 @@ __global__ __launch_bounds__(64 * WM * WN) void w4_gemm_kernel(W4Args a, int mb,
 
   // Loads never depend on a branch, so that the compiler waits for those it needs and no more: the last steps load the
   // last one again.
-  load_x(0);
+  load_x(4 * kg);
 #pragma unroll
   for (int j = 0; j < 4; j++) {
-    load_piece(0, j);
+    load_piece(8 * kg, j);
     put_piece(0, j);
   }
-  load_piece(1, 0);
-  put_x(0);
-  load_x(steps > 1 ? 1 : 0);
+  load_piece(8 * (kg + KG), 0);
+  put_x(4 * kg);
+  load_x(4 * kg + 1);
   __syncthreads();
-  for (int S = 0; 4 * S < steps; S++) {
+  int S = kg;
+  for (int four = 0; 4 * (S - kg) < steps; S += KG, four ^= 1) {  // of several groups all go on to the end, with zeros of x
     u2v scale[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      scale[t] = *reinterpret_cast<const u2v*>(&scales_lds[S & 1][((wn * NT + t) * 32 + i) * 8]);
+      scale[t] = *reinterpret_cast<const u2v*>(&L.scales[four][((wn * NT + t) * 32 + i) * 8]);
       scale[t][0] >>= 8 * h, scale[t][1] >>= 8 * h;
     }
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const int s = 4 * S + j;
-      if (s >= steps) break;
-      const u8* buf = lds[s & 1];
+      if (KG == 1 && 4 * S + j >= steps) break;
+      const u8* buf = L.x[j & 1];
       v8 x[2][2];
       w4_u4 codes[NT];
 #pragma unroll
       for (int q = 0; q < 2; q++) x[0][q] = *reinterpret_cast<const v8*>(buf + from[q]);
 #pragma unroll
-      for (int t = 0; t < NT; t++) codes[t] = *reinterpret_cast<const w4_u4*>(&codes_lds[S & 1][code_from[t] ^ (j * 32)]);
+      for (int t = 0; t < NT; t++) codes[t] = *reinterpret_cast<const w4_u4*>(&L.codes[four][code_from[t] ^ (j * 32)]);
       // what the next step, or the next four, will read has had a whole step to arrive; its place was last read before a barrier
-      put_x(s + 1);
-      put_piece(S + 1, j);
-      load_x(s + 2 < steps ? s + 2 : steps - 1);
-      load_piece(j < 3 ? S + 1 : S + 2, (j + 1) & 3);
+      put_x(j < 3 ? 4 * S + j + 1 : 4 * (S + KG));
+      put_piece(four ^ 1, j);
+      load_x(j < 2 ? 4 * S + j + 2 : 4 * (S + KG) + j - 2);
+      load_piece(8 * (j < 3 ? S + KG : S + 2 * KG), (j + 1) & 3);
       __builtin_amdgcn_sched_barrier(0);  // on their way now, not where the registers are short
 #pragma unroll
       for (int t = 0; t < 4; t++) {
@@ -149,6 +161,37 @@ __global__ __launch_bounds__(64 * WM * WN) void w4_gemm_kernel(W4Args a, int mb,
       }
       __syncthreads();
     }
+  }
+  if constexpr (KG > 1) {  // add up: every wave's sums in LDS, four outputs of a row to a thread
+    f4v* sums = reinterpret_cast<f4v*>(shared);
+    auto slot = [&](int g, int w, int q, int t, int r) W4_AI { return ((((g * WAVES + w) * 2 + q) * NT + t) * 4 + r) * 64; };
+#pragma unroll
+    for (int q = 0; q < 2; q++)
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          sums[slot(kg, wave, q, t, r) + lane] = f4v{acc[q][t][4 * r], acc[q][t][4 * r + 1], acc[q][t][4 * r + 2], acc[q][t][4 * r + 3]};
+    __syncthreads();
+    auto sum = [&](int at) W4_AI {
+      f4v v = sums[at];
+#pragma unroll
+      for (int g = 1; g < KG; g++) v += sums[at + slot(g, 0, 0, 0, 0)];
+      return v;
+    };
+    constexpr int COLS = GATED && !PAIRED ? WN / 2 : WN;  // of waves with outputs
+    for (int e = threadIdx.x; e < WM * COLS * 2 * OT * 256; e += KG * THREADS) {
+      const int l = e % 64, r = e / 64 % 4, t = e / 256 % OT, q = e / (256 * OT) % 2, w = e / (512 * OT), col = w % COLS, row = w / COLS;
+      f4v v = sum(slot(0, row * WN + col, q, t, r) + l);
+      if (GATED) {
+        const f4v u = sum((PAIRED ? slot(0, row * WN + col, q, OT + t, r) : slot(0, row * WN + col + COLS, q, t, r)) + l);
+#pragma unroll
+        for (int c = 0; c < 4; c++) v[c] = w4_silu(v[c]) * u[c];
+      }
+      const int m = m0 + row * 64 + 32 * q + l % 32, n = n0 + (col * OT + t) * 32 + 8 * r + 4 * (l / 32);
+      if (m < a.M && n < a.F) w4_store<T>(a, m, n, v);
+    }
+    return;
   }
   auto value = [&](int q, int t, int r) W4_AI {
     f4v v = {acc[q][t][4 * r], acc[q][t][4 * r + 1], acc[q][t][4 * r + 2], acc[q][t][4 * r + 3]};
@@ -174,8 +217,8 @@ __global__ __launch_bounds__(64 * WM * WN) void w4_gemm_kernel(W4Args a, int mb,
   // 32 rows of this wave's outputs at a time through its own part of LDS, so that a row's bytes leave together
   typedef T v4 __attribute__((ext_vector_type(4)));
   constexpr int ROW = 64 * OT, PER = ROW / 16;  // bytes, 16-byte chunks of a row
-  static_assert(WAVES * 32 * ROW <= (int)sizeof lds, "the waves' parts fit");
-  u8* part = &lds[0][0] + wave * 32 * ROW;
+  static_assert(WAVES * 32 * ROW <= (int)sizeof shared, "the waves' parts fit");
+  u8* part = shared + wave * 32 * ROW;
 #pragma unroll
   for (int q = 0; q < 2; q++) {
 #pragma unroll
@@ -194,20 +237,52 @@ __global__ __launch_bounds__(64 * WM * WN) void w4_gemm_kernel(W4Args a, int mb,
   }
 }
 
-template <class T, int WM, int WN, int NT, bool GATED>
+template <class T, int KG, int WM, int WN, int NT, bool GATED>
 int launch(const char* fn, const W4Args& a, hipStream_t stream) {
-  constexpr int BM = 64 * WM, BN = 32 * (GATED ? NT / 2 : NT) * WN;
+  constexpr int BM = 64 * WM, BN = 32 * NT * WN / (GATED ? 2 : 1), THREADS = 64 * KG * WM * WN;
   const long mb = ((long)a.M + BM - 1) / BM, nb = ((long)a.F + BN - 1) / BN, blocks = (mb * nb + 7) / 8 * 8;
-  if (blocks > 0x7fffffffL / (64 * WM * WN)) return uwc_fail("%s: too many rows (%d) and outputs (%d)", fn, a.M, a.F);
-  hipLaunchKernelGGL((w4_gemm_kernel<T, WM, WN, NT, GATED>), dim3((unsigned)blocks), dim3(64 * WM * WN), 0, stream, a, (int)mb, (int)nb);
+  if (blocks > 0x7fffffffL / THREADS) return uwc_fail("%s: too many rows (%d) and outputs (%d)", fn, a.M, a.F);
+  hipLaunchKernelGGL((w4_gemm_kernel<T, KG, WM, WN, NT, GATED>), dim3((unsigned)blocks), dim3(THREADS), 0, stream, a, (int)mb, (int)nb);
   return uwc_launch_status(fn);
+}
+
+// us that a round of tiles, one to a compute unit, spends on a step of a group: of one tile alone, and with all units at work (power, L2).
+// Measured over K = 4096 at 64 to 2048 rows of 4096 weights, and at 8192 rows; whole calls come within 15% of what they say
+// (512 x 4096 x 4096: 78, 52, 36, 26 and 34 us in the forms' order; 1024: 79, 55, 43, 53, 64; 2048: 86, 73, 86, 100, 125).
+struct Form {
+  int BM, rows, KG;
+  float alone, full;
+};
+const Form forms[] = {{256, 256, 1, 1.19f, 1.6f}, {128, 256, 1, 0.8f, 1.15f}, {128, 128, 2, 1.03f, 1.34f}, {64, 128, 2, 0.69f, 0.78f}, {64, 64, 4, 1.05f, 0.97f}};
+
+int choose(const W4Args& a, bool gated) {
+  const long cus = uwc_cu_count(), steps = (a.K + 63) / 64;
+  int best = 0;
+  float least = 0;
+  for (int f = 0; f < 5; f++) {
+    const Form& F = forms[f];
+    const long out = F.rows / (gated ? 2 : 1), tiles = (((long)a.M + F.BM - 1) / F.BM) * ((a.F + out - 1) / out), rest = tiles % cus;
+    const float rounds = tiles / cus * F.full + (rest ? F.alone + (F.full - F.alone) * rest / cus : 0);
+    const float us = rounds * ((steps + 4 * F.KG - 1) / (4 * F.KG) * 4);
+    if (!f || us < least) best = f, least = us;
+  }
+  return best;
+}
+
+template <class T, bool GATED>
+int run(const char* fn, const W4Args& a, hipStream_t stream) {
+  switch (choose(a, GATED)) {
+    case 0: return launch<T, 1, 4, 2, 4, GATED>(fn, a, stream);
+    case 1: return launch<T, 1, 2, 4, 2, GATED>(fn, a, stream);
+    case 2: return launch<T, 2, 2, 2, 2, GATED>(fn, a, stream);
+    case 3: return launch<T, 2, 1, 4, 1, GATED>(fn, a, stream);
+    default: return launch<T, 4, 1, 2, 1, GATED>(fn, a, stream);
+  }
 }
 
 }  // namespace
 
-bool w4_gemm_pays(int M, int F, int K, bool gated) { return M > 128; }
-
 int w4_gemm(const char* fn, const W4Args& a, int dtype, bool gated, hipStream_t stream) {
-  if (dtype == UWC_W4_BF16) return gated ? launch<__bf16, 4, 2, 4, true>(fn, a, stream) : launch<__bf16, 4, 2, 4, false>(fn, a, stream);
-  return gated ? launch<_Float16, 4, 2, 4, true>(fn, a, stream) : launch<_Float16, 4, 2, 4, false>(fn, a, stream);
+  if (dtype == UWC_W4_BF16) return gated ? run<__bf16, true>(fn, a, stream) : run<__bf16, false>(fn, a, stream);
+  return gated ? run<_Float16, true>(fn, a, stream) : run<_Float16, false>(fn, a, stream);
 }
