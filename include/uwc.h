@@ -466,6 +466,32 @@ int uwc_kv_read(const int8_t* k, const int8_t* v, const float* ks, const float* 
                 int hd, const int32_t* table, int64_t table_stride, int width, const int32_t* start, const int32_t* cu,
                 int B, int rows, int dtype, void* ko, void* vo, hipStream_t stream);
 
+/* Pages of a cache that sequences share. refs (int32, pages): how many hold a page, rows of the table and others; one
+ * with none is free. caches: a HOST array of 4 * layers device pointers, k, v, ks and vs of each layer, all of the same shape;
+ * every layer uses the same pages. At most 8192 rows, 2^22 pages. New tables (R or B rows of `width` entries, dense), lengths and
+ * counts are outputs of their own and overlap no input; the caches change in place. scratch: uwc_kv_pages_scratch_bytes(pages, R) bytes
+ * (compact: R = 0), 16-byte aligned, no contents kept between calls. Entries outside [0, pages) are pages that are not
+ * there: they are kept as they are and counted nowhere. */
+uint64_t uwc_kv_pages_scratch_bytes(int64_t pages, int rows);
+
+/* Row i of the new table continues old row parents[i], of lens[parents[i]] tokens, or is empty (-1 in every entry, length 0)
+ * where parents[i] is outside [0, B). The first row of a parent keeps all its entries, the others those of its full pages.
+ * The last page, where it is partly filled and there, is copied in every layer for the others, and for the first too if refs says
+ * that more than one hold it: its first slots, up to a multiple of 16, and scales. Then every row gets pages up to
+ * lens + room tokens (and the table's width). Pages are taken from those without a holder after all old rows that nobody
+ * continues have let theirs go: the lowest first, by rows, by entries. Where they run out, entries are -1 and *missing
+ * is how many. */
+int uwc_kv_fork(int layers, void* const* caches, int64_t pages, int page, int Hkv, int hd, const int32_t* table,
+                int64_t table_stride, int width, const int32_t* lens, int B, const int32_t* refs, const int32_t* parents, int R,
+                int room, int32_t* new_table, int32_t* new_lens, int32_t* new_refs, int32_t* missing, void* scratch,
+                uint64_t scratch_bytes, hipStream_t stream);
+
+/* With n pages held: those from n on move, in their order, to the free ones below n, in every layer; the new table and
+ * counts name them there, and no page from n on is held. */
+int uwc_kv_compact(int layers, void* const* caches, int64_t pages, int page, int Hkv, int hd, const int32_t* table,
+                   int64_t table_stride, int width, int B, const int32_t* refs, int32_t* new_table, int32_t* new_refs,
+                   void* scratch, uint64_t scratch_bytes, hipStream_t stream);
+
 /* ======================================================================== linears with 4-bit weights
  * Weights in the OCP microscaling format of fp4 elements, rows in 16 bits (UWC_W4_BF16 or UWC_W4_FP16). No counterpart
  * in the reference (its linears are 8-bit, runtime/detrt/qwen3.py:71-126).

@@ -77,13 +77,16 @@ SIGNATURES = {
     "uwc_kv_attend": [vp, vp, vp, vp, i64, i32, i32, i32, vp, i64, i32, i32, i32, vp, i64, i32, vp, vp, i32, i32, i32, i32, i32,
                       f32, vp, u64, vp, vp],
     "uwc_kv_read": [vp, vp, vp, vp, i64, i32, i32, i32, vp, i64, i32, vp, vp, i32, i32, i32, vp, vp, vp],
+    "uwc_kv_pages_scratch_bytes": [i64, i32],
+    "uwc_kv_fork": [i32, vp, i64, i32, i32, i32, vp, i64, i32, vp, i32, vp, vp, i32, i32, vp, vp, vp, vp, vp, u64, vp],
+    "uwc_kv_compact": [i32, vp, i64, i32, i32, i32, vp, i64, i32, i32, vp, vp, vp, vp, u64, vp],
     "uwc_w4_linear": [vp, i64, i32, i32, vp, vp, i32, i32, vp, vp, vp],
     "uwc_w4_gated": [vp, i64, i32, i32, vp, vp, i32, i32, vp, vp],
     "uwc_mfma_rate_probe": [i32, i32, vp, i64, vp],
 }
 _RESTYPE = {"uwc_last_error": ctypes.c_char_p, "uwc_header_sha": ctypes.c_char_p,
             "uwc_attention_scratch_bytes": ctypes.c_uint64, "uwc_decoder_layer_scratch_bytes": ctypes.c_uint64,
-            "uwc_kv_attend_scratch_bytes": ctypes.c_uint64}
+            "uwc_kv_attend_scratch_bytes": ctypes.c_uint64, "uwc_kv_pages_scratch_bytes": ctypes.c_uint64}
 
 _LIB = None
 
@@ -142,18 +145,18 @@ _KV = None
 
 
 class _LongWay:
-    """Stands in for _kv.so: every call is left to what follows it in kv.py."""
+    """Stands in for _kv.so: every call is left to what follows it in kv.py, pages.py or w4.py."""
 
     @staticmethod
     def append(*args):
         return None
 
-    attend = read = append
+    attend = read = fork = compact = linear = gated = append
 
 
 def kv():
-    """_kv.so (uwc_kv_bind.cpp), the short way to the key/value cache's entry points, bound to the
-    library; it has to be built from the same header. Where it is not built or does not fit this torch, calls go
+    """_kv.so (uwc_kv_bind.cpp), the short way to the entry points of the key/value cache, its pages and the linears with 4-bit
+    weights, bound to the library; it has to be built from the same header. Where it is not built or does not fit this torch, calls go
     through ctypes."""
     global _KV
     if _KV is None:
@@ -161,8 +164,8 @@ def kv():
         try:
             from . import _kv
         except ImportError as e:
-            warnings.warn(f"{os.path.join(_HERE, '_kv.so')} is not built or does not fit this torch ({e}): calls of uwc_amd.kv "
-                          "take some 10 us longer each. To build it, run useful-work-coin_amd/csrc/build.sh "
+            warnings.warn(f"{os.path.join(_HERE, '_kv.so')} is not built or does not fit this torch ({e}): calls of uwc_amd.kv, "
+                          "pages and w4 take some 10 us longer each. To build it, run useful-work-coin_amd/csrc/build.sh "
                           "(or __graft_entry__.build())", RuntimeWarning, stacklevel=3)
             _KV = _LongWay
             return _KV
@@ -170,6 +173,7 @@ def kv():
             raise ImportError("_kv.so and libuwc_hip.so were built from different include/uwc.h: rebuild with "
                               "useful-work-coin_amd/csrc/build.sh (or __graft_entry__.build())")
         _kv.bind(*(ctypes.cast(f, vp).value for f in (L.uwc_kv_append, L.uwc_kv_attend_scratch_bytes, L.uwc_kv_attend,
-                                                      L.uwc_kv_read)))
+                                                      L.uwc_kv_read, L.uwc_kv_pages_scratch_bytes, L.uwc_kv_fork,
+                                                      L.uwc_kv_compact, L.uwc_w4_linear, L.uwc_w4_gated)))
         _KV = _kv
     return _KV

@@ -16,13 +16,14 @@ Rows x are bfloat16 or float16, sums fp32, rounded once to x's type. bfloat16 ro
 float16 rows the weights are rounded to float16 (exact for scales from 103 to 140; of larger ones those past 65504 are infinite).
 A scale of 255 is not a number: its row's outputs are NaN. Nothing is recorded for autograd.
 
-Everything runs on torch's current HIP stream; buffers are torch tensors on the caller's GPU.
+Everything runs on torch's current HIP stream; buffers are torch tensors on the caller's GPU. Arguments of the usual form
+take the short way of uwc_amd.kv.
 """
 from __future__ import annotations
 
 import torch
 
-from . import _lib
+from . import _lib, kv
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1}
 GROUP = 32
@@ -105,6 +106,9 @@ def _call(fn, x, codes, scales):
 
 def linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bias=None) -> torch.Tensor:
     """x W^T (+ bias): (..., N) in x's type, for x (..., K); bias (N,) in x's type."""
+    r = _lib.kv().linear(x, codes, scales, bias, kv._stream())
+    if r is not None:
+        return r if type(r) is not int else _lib.fail("uwc_w4_linear", r)
     fn = "w4.linear"
     rows, N, K = _call(fn, x, codes, scales)
     if bias is not None:
@@ -120,6 +124,9 @@ def linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bias=None
 
 def gated(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     """silu(x G^T) * (x U^T): (..., F) in x's type; the weight's first F rows are G, the other F are U."""
+    r = _lib.kv().gated(x, codes, scales, kv._stream())
+    if r is not None:
+        return r if type(r) is not int else _lib.fail("uwc_w4_gated", r)
     fn = "w4.gated"
     rows, N, K = _call(fn, x, codes, scales)
     _require(N % 2 == 0, f"{fn}: the weight's rows are a gate's and as many of the other projection, got {N}")
