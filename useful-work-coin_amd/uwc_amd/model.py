@@ -14,6 +14,9 @@ the exact int8 GEMM, so every mode below except "bf16" produces the same bits.
   "mined"  MinedWeight.forward: commitment, noise, hashed GEMM and exact denoise, for mineable
            shapes.
 A shape that cannot be mined runs the "int" math in every integer mode.
+
+For serving without the integer math's exactness, convert_4bit puts linears with 4-bit weights (uwc_amd.w4) in their place,
+a feed-forward block's gate, up, activation and product in one kernel.
 """
 from __future__ import annotations
 
@@ -23,7 +26,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import ops
+from . import ops, w4
 
 QMAX = 64
 MODES = ("bf16", "int", "plain", "mined")
@@ -243,4 +246,69 @@ def convert_qwen3(model, device, mode="mined", hadamard_block=512, mine_lm_head=
             out.append(_fuse(parent, group, device, mode, hadamard_block, cfg))
     if mine_lm_head and hasattr(model, "lm_head"):
         out.append(_fuse(model, ["lm_head"], device, mode, hadamard_block, cfg))
+    return out
+
+
+class FourBitLinear(nn.Module):
+    """One nn.Linear, or several that read the same input concatenated along n, with weights of 4 bits (uwc_amd.w4).
+    `splits` are the fused layers' output widths. Rows keep their type, bfloat16 or float16."""
+
+    def __init__(self, linears: list[nn.Linear], device):
+        super().__init__()
+        self.splits = [lin.out_features for lin in linears]
+        self.k, self.n = linears[0].in_features, sum(self.splits)
+        parts = [w4.quantize(lin.weight.detach().to(device)) for lin in linears]
+        self.register_buffer("codes", torch.cat([c for c, _ in parts]))
+        self.register_buffer("scales", torch.cat([s for _, s in parts]))
+        bias = None
+        if any(lin.bias is not None for lin in linears):
+            bias = torch.cat([(lin.bias.detach() if lin.bias is not None else lin.weight.new_zeros(lin.out_features)).to(device) for lin in linears])
+        self.register_buffer("bias", bias)
+
+    @torch.compiler.disable
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return w4.linear(x, self.codes, self.scales, self.bias)
+
+
+class FourBitMLP(nn.Module):
+    """down(silu(gate(x)) * up(x)) with weights of 4 bits: two kernels."""
+
+    def __init__(self, mlp: nn.Module, device):
+        super().__init__()
+        self.check(mlp)
+        self.gate_up, self.down = FourBitLinear([mlp.gate_proj, mlp.up_proj], device), FourBitLinear([mlp.down_proj], device)
+
+    @staticmethod
+    def check(mlp: nn.Module):
+        if mlp.gate_proj.bias is not None or mlp.up_proj.bias is not None:
+            raise AssertionError("FourBitMLP: gate and up projections must have no bias")
+        z = torch.linspace(-4, 4, 33)
+        if not torch.allclose(mlp.act_fn(z), F.silu(z), rtol=1e-5, atol=1e-6):
+            raise AssertionError("FourBitMLP: the activation must be silu")
+
+    @torch.compiler.disable
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return self.down(w4.gated(x, self.gate_up.codes, self.gate_up.scales))
+
+
+def convert_4bit(model, device, lm_head: bool = False) -> list[nn.Module]:
+    """Replace the linears of a Hugging Face Qwen3 or Llama model (a CausalLM or the bare model), in bfloat16 or float16, by
+    FourBitLinears, q/k/v fused and each feed-forward block a FourBitMLP; returns them per layer (qkv, o, feed-forward), then
+    the lm_head where it is asked for. The weights are rounded to 4 bits as they are, without calibration."""
+    decoder = getattr(model, "model", model)
+    for layer in decoder.layers:  # before anything is replaced
+        FourBitMLP.check(layer.mlp)
+    out = []
+    for layer in decoder.layers:
+        att = layer.self_attn
+        qkv = FourBitLinear([att.q_proj, att.k_proj, att.v_proj], device)
+        shared = _SharedOutput(qkv)
+        for i, name in enumerate(("q_proj", "k_proj", "v_proj")):
+            setattr(att, name, _Part(shared, i))
+        att.o_proj = FourBitLinear([att.o_proj], device)
+        layer.mlp = FourBitMLP(layer.mlp, device)
+        out += [qkv, att.o_proj, layer.mlp]
+    if lm_head and hasattr(model, "lm_head"):
+        model.lm_head = FourBitLinear([model.lm_head], device)
+        out.append(model.lm_head)
     return out
