@@ -198,7 +198,8 @@ __device__ __forceinline__ void put_range(const Scratch& s, int range, int pages
 }
 
 __global__ __launch_bounds__(256) void fork_plan_kernel(ForkArgs a, int ranges) {
-  __shared__ int children[ROWS], change[RANGE], tmp[4];
+  __shared__ int children[ROWS], change[RANGE], tmp[4], listed;
+  __shared__ unsigned short list[ROWS];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   auto length = [&](int r) KV_AI {
     const int n = a.lens[r];
@@ -215,14 +216,27 @@ __global__ __launch_bounds__(256) void fork_plan_kernel(ForkArgs a, int ranges) 
       if (r >= 0 && r < a.B) atomicAdd(&children[r], 1);
     }
     __syncthreads();
-    for (int r = wave; r < a.B; r += 4) {
-      const int c = children[r];
-      if (c == 1) continue;
-      const int full = c ? length(r) / a.page : a.width;
-      for (int j = lane; j < full; j += 64) {
-        const int p = a.table[r * a.stride + j];
-        if (p >= p0 && p < p0 + RANGE && p < a.pages) atomicAdd(&change[p - p0], c - 1);
+    // the rows whose pages change hands, in any order: they are added up; then all their entries, eight to a thread on their way
+    if (t == 0) listed = 0;
+    __syncthreads();
+    for (int r = t; r < a.B; r += 256)
+      if (children[r] != 1) list[atomicAdd(&listed, 1)] = (unsigned short)r;
+    __syncthreads();
+    const long entries = (long)listed * a.width;
+    for (long e0 = t; e0 < entries; e0 += 256 * 8) {
+      int p[8], c[8];
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const long e = e0 + 256 * k < entries ? e0 + 256 * k : entries - 1;
+        const u32 at = (u32)(e / a.width), j = (u32)(e - (long)at * a.width);
+        const int r = list[at];
+        p[k] = a.table[r * a.stride + j];
+        c[k] = children[r] ? (int)j < length(r) / a.page ? children[r] - 1 : 0 : -1;
+        if (e0 + 256 * k >= entries) c[k] = 0;
       }
+#pragma unroll
+      for (int k = 0; k < 8; k++)
+        if (c[k] && p[k] >= p0 && p[k] < p0 + RANGE && p[k] < a.pages) atomicAdd(&change[p[k] - p0], c[k]);
     }
     __syncthreads();
     put_range(a.s, blockIdx.x, a.pages, tmp, [&](int p) KV_AI {
@@ -378,9 +392,10 @@ int by_layers(const char* fn, int layers, void* const* caches, int Hkv, int hd, 
   return UWC_OK;
 }
 
-// Workgroups of the second launch: as many as there can be jobs, up to eight to a compute unit, which then take several each.
-unsigned grid_of(long jobs, long rows) {
-  const long most = 8L * uwc_cu_count(), n = jobs > rows ? jobs : rows;
+// Workgroups of the second launch: as many as there can be jobs, up to what the compute units hold at once, which then take several
+// each (fork: 64 KB of LDS, two to a unit; four rounds of them, each finding its rows' ranks, took 10.5 us where nothing is copied).
+unsigned grid_of(int to_a_unit, long jobs, long rows) {
+  const long most = (long)to_a_unit * uwc_cu_count(), n = jobs > rows ? jobs : rows;
   return (unsigned)(n < 1 ? 1 : n < most ? n : most);
 }
 
@@ -408,7 +423,7 @@ extern "C" int uwc_kv_fork(int layers, void* const* caches, int64_t pages, int p
   hipLaunchKernelGGL(fork_plan_kernel, dim3(ranges + R), dim3(256), 0, stream, a, ranges);
   if (int st = uwc_launch_status(fn)) return st;
   return by_layers(fn, layers, caches, Hkv, hd, page, [&](const Layers& L, bool first) {
-    hipLaunchKernelGGL(fork_finish_kernel, dim3(grid_of(R * pieces_on_host(Hkv, page, hd) * L.n, R)), dim3(256), 0, stream, a, L, ranges, first);
+    hipLaunchKernelGGL(fork_finish_kernel, dim3(grid_of(2, R * pieces_on_host(Hkv, page, hd) * L.n, R)), dim3(256), 0, stream, a, L, ranges, first);
   });
 }
 
@@ -425,6 +440,6 @@ extern "C" int uwc_kv_compact(int layers, void* const* caches, int64_t pages, in
   return by_layers(fn, layers, caches, Hkv, hd, page, [&](const Layers& L, bool first) {
     // at most half of the pages move
     const long jobs = pages / 2 * pieces_on_host(Hkv, page, hd) * L.n, rows = (pages + (long)B * width + 255) / 256;
-    hipLaunchKernelGGL(compact_finish_kernel, dim3(grid_of(jobs, rows)), dim3(256), 0, stream, a, L, ranges, first);
+    hipLaunchKernelGGL(compact_finish_kernel, dim3(grid_of(8, jobs, rows)), dim3(256), 0, stream, a, L, ranges, first);
   });
 }
