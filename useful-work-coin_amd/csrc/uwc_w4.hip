@@ -87,7 +87,7 @@ __global__ __launch_bounds__(64 * W) void w4_rows_kernel(W4Args a, int nb, int m
         for (int q = 0; q < MT; q++) acc[q][n] = W4<T>::mul(w, r.x[q][t], acc[q][n]);
       }
   };
-  // the next unit's weights, and for few rows its x, are on their way while this one is multiplied
+  // the next unit's weights are on their way while this one is multiplied; its x too where one tile a wave leaves registers for that
   int u = wave;
   if (u < units) {
     Weights now;
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(64 * W) void w4_rows_kernel(W4Args a, int nb, int m
     for (; u + W < units; u += W) {
       Weights next;
       load(next, u + W);
-      if constexpr (MT == 1) {
+      if constexpr (MT == 1 && NT == 1) {
         Rows nx;
         load_rows(nx, u + W);
         mul(now, x);
@@ -144,12 +144,17 @@ int rows(const char* fn, const W4Args& a, hipStream_t stream) {
   return uwc_launch_status(fn);
 }
 
-// More tiles of weights to a workgroup share the loads of x, fewer keep all compute units at work.
+// More tiles of weights to a workgroup share the loads of x, which take longer than the codes from about four rows on (64 lines of
+// memory an instruction against 16); fewer, and more waves to a tile, keep all compute units at work. us, weights from HBM:
+//   gated, tiles x waves    2 x 4   4 x 4   2 x 8        linear                  1 x 8   2 x 8   4 x 4
+//   1 x 14336 x 4096         18.2    19.4    19.8        1 x 4096 x 14336         13.2    19.4    50.2
+//   16 x 14336 x 4096        40.1    25.2    39.9        13 x 6144 x 4096         12.3     8.9    12.8
+//   1 x 6144 x 2048           6.5     7.6     6.8        8 x 28672 x 4096         32.1    25.5    20.5
 template <class T>
 int run(const char* fn, const W4Args& a, bool gated, hipStream_t stream) {
-  if (gated) return a.F >= 8192 || a.M > 4 ? rows<T, 1, 4, 4, true>(fn, a, stream) : rows<T, 1, 2, 4, true>(fn, a, stream);
+  if (gated) return a.M > 4 ? rows<T, 1, 4, 4, true>(fn, a, stream) : rows<T, 1, 2, 4, true>(fn, a, stream);
   if (a.M > 16) return rows<T, 2, 1, 8, false>(fn, a, stream);
-  if (a.F >= 16384) return rows<T, 1, 2, 4, false>(fn, a, stream);
+  if (a.F >= 16384) return rows<T, 1, 4, 4, false>(fn, a, stream);
   if (a.F >= 6144) return rows<T, 1, 2, 8, false>(fn, a, stream);
   return rows<T, 1, 1, 8, false>(fn, a, stream);
 }
@@ -163,6 +168,8 @@ int call(const char* fn, const W4Args& a, int dtype, bool gated, hipStream_t str
   if (a.x_stride > 1 << 22) return uwc_fail("%s: rows of x are %ld elements apart, more than 2^22", fn, a.x_stride);
   if (a.x_stride < 0 || a.x_stride % 8 || (((uintptr_t)a.x | (uintptr_t)a.codes) & 15) || ((uintptr_t)a.y & 7))
     return uwc_fail("%s: rows of x and codes must be 16-byte aligned, y 8-byte aligned", fn);
+  // the tiles in LDS from 17 rows on (24 x 6144 x 2048, gated: 13.8 us here, 11.7 there), of fewer weights from 33
+  // (24 x 4096 x 4096: 11.5 here, 16.5 there)
   if (a.M > (gated || a.F > 8192 ? 16 : 32)) return w4_gemm(fn, a, dtype, gated, stream);
   return dtype == UWC_W4_BF16 ? run<__bf16>(fn, a, gated, stream) : run<_Float16>(fn, a, gated, stream);
 }

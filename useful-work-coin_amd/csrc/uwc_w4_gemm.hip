@@ -90,12 +90,12 @@ __global__ __launch_bounds__(64 * KG * WM * WN) void w4_gemm_kernel(W4Args a, in
   };
   // piece j of four steps: of their eight groups, from `first` on, the codes of the j-th quarter of the rows, and bytes j and 4 + j of
   // every row's scales; groups past the last are the last, and meet zeros of x
-  auto load_piece = [&](int first, int j) W4_AI {
+  auto load_piece = [&](int first, int j, w4_u4& piece, u32& scale_byte) W4_AI {
     const int g = first + chunk, e = first + 4 * (tid & 1) + j;
     piece = *reinterpret_cast<const w4_u4*>(code_at[j] + (g < groups ? g : groups - 1) * 16);
     scale_byte = scale_at[e < groups ? e : groups - 1];
   };
-  auto put_piece = [&](int buf, int j) W4_AI {
+  auto put_piece = [&](int buf, int j, const w4_u4& piece, u32 scale_byte) W4_AI {
     const int r = j * (ROWS / 4) + (tid >> 3);
     *reinterpret_cast<w4_u4*>(&L.codes[buf][r * 128 + ((chunk ^ (r >> 1)) & 7) * 16]) = piece;
     L.scales[buf][(tid >> 1) * 8 + 4 * (tid & 1) + j] = (u8)scale_byte;
@@ -110,15 +110,19 @@ __global__ __launch_bounds__(64 * KG * WM * WN) void w4_gemm_kernel(W4Args a, in
 
   // Loads never depend on a branch, so that the compiler waits for those it needs and no more: the last steps load the
   // last one again.
-  load_x(4 * kg);
+  {
+    w4_u4 first[4];
+    u32 bytes[4];
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    load_piece(8 * kg, j);
-    put_piece(0, j);
+    for (int j = 0; j < 4; j++) load_piece(8 * kg, j, first[j], bytes[j]);
+    load_x(4 * kg);
+    load_piece(8 * (kg + KG), 0, piece, scale_byte);
+    __builtin_amdgcn_sched_barrier(0);  // all on their way at once
+#pragma unroll
+    for (int j = 0; j < 4; j++) put_piece(0, j, first[j], bytes[j]);
+    put_x(4 * kg);
+    load_x(4 * kg + 1);
   }
-  load_piece(8 * (kg + KG), 0);
-  put_x(4 * kg);
-  load_x(4 * kg + 1);
   __syncthreads();
   int S = kg;
   for (int four = 0; 4 * (S - kg) < steps; S += KG, four ^= 1) {  // of several groups all go on to the end, with zeros of x
@@ -134,21 +138,23 @@ __global__ __launch_bounds__(64 * KG * WM * WN) void w4_gemm_kernel(W4Args a, in
       const u8* buf = L.x[j & 1];
       v8 x[2][2];
       w4_u4 codes[NT];
+      auto read_x = [&](int t) W4_AI {
 #pragma unroll
-      for (int q = 0; q < 2; q++) x[0][q] = *reinterpret_cast<const v8*>(buf + from[q]);
+        for (int q = 0; q < 2; q++) x[t & 1][q] = *reinterpret_cast<const v8*>(buf + (from[q] ^ (t * 16)));
+      };
+      read_x(0);
 #pragma unroll
       for (int t = 0; t < NT; t++) codes[t] = *reinterpret_cast<const w4_u4*>(&L.codes[four][code_from[t] ^ (j * 32)]);
       // what the next step, or the next four, will read has had a whole step to arrive; its place was last read before a barrier
       put_x(j < 3 ? 4 * S + j + 1 : 4 * (S + KG));
-      put_piece(four ^ 1, j);
+      put_piece(four ^ 1, j, piece, scale_byte);
       load_x(j < 2 ? 4 * S + j + 2 : 4 * (S + KG) + j - 2);
-      load_piece(8 * (j < 3 ? S + KG : S + 2 * KG), (j + 1) & 3);
+      load_piece(8 * (j < 3 ? S + KG : S + 2 * KG), (j + 1) & 3, piece, scale_byte);
       __builtin_amdgcn_sched_barrier(0);  // on their way now, not where the registers are short
 #pragma unroll
       for (int t = 0; t < 4; t++) {
         if (t < 3) {
-#pragma unroll
-          for (int q = 0; q < 2; q++) x[(t + 1) & 1][q] = *reinterpret_cast<const v8*>(buf + (from[q] ^ ((t + 1) * 16)));
+          read_x(t + 1);
           __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
