@@ -169,17 +169,19 @@ __device__ __forceinline__ void copy(const Layers& L, int layer, int piece, int 
   }
 }
 
-// This workgroup's share of `moves` pages in all layers, piece by piece: each(move, layer, piece).
-template <class F>
-__device__ __forceinline__ void share(const Layers& L, int moves, F&& each) {
-  const u32 pieces = pieces_of(L), per = L.n * pieces;
-  if (!per) return;
-  u32 move = blockIdx.x / per, rest = blockIdx.x % per;
-  const u32 on = gridDim.x / per, more = gridDim.x % per;
-  while (move < (u32)moves) {
-    each((int)move, uniform(rest / pieces), uniform(rest % pieces));
-    move += on, rest += more;
-    if (rest >= per) rest -= per, move++;
+// This workgroup's share of `moves` pages in all layers: find(move) once for each move it works on, then each(layer, piece). Where there
+// are fewer moves than workgroups, several share one (a search for each piece took 59 us for 350 small pages in 18 layers).
+template <class S, class F>
+__device__ __forceinline__ void share(const Layers& L, int moves, S&& find, F&& each) {
+  const int pieces = pieces_of(L), per = L.n * pieces, groups = gridDim.x;
+  if (!per || !moves) return;
+  const int to_a_move = moves >= groups ? 1 : groups / moves < per ? groups / moves : per, at_once = groups / to_a_move;
+  const int part = uniform(blockIdx.x % to_a_move);
+  int move = uniform(blockIdx.x / to_a_move);
+  if (move >= at_once) return;  // what is left over of the workgroups
+  for (; move < moves; move += at_once) {
+    find(move);
+    for (int rest = part; rest < per; rest += to_a_move) each(uniform(rest / pieces), uniform(rest % pieces));
   }
 }
 
@@ -314,11 +316,13 @@ __global__ __launch_bounds__(256) void fork_finish_kernel(ForkArgs a, Layers L, 
       }
     }
   }
-  share(L, n, [&](int move, int layer, int piece) KV_AI {
+  int src = 0, dst = 0, granules = 0;
+  share(L, n, [&](int move) KV_AI {
     const int i = copies[move];
     const Row r = a.s.rows[i];
-    copy(L, layer, piece, uniform(r.tail < -1 ? -2 - r.tail : r.tail), uniform(select<true>(sums, ranges, a.s.bits, rank[i])), uniform(r.granules));
-  });
+    src = uniform(r.tail < -1 ? -2 - r.tail : r.tail), granules = uniform(r.granules);
+    dst = uniform(select<true>(sums, ranges, a.s.bits, rank[i]));
+  }, [&](int layer, int piece) KV_AI { copy(L, layer, piece, src, dst, granules); });
 }
 
 __global__ __launch_bounds__(256) void compact_plan_kernel(CompactArgs a) {
@@ -345,9 +349,10 @@ __global__ __launch_bounds__(256) void compact_finish_kernel(CompactArgs a, Laye
       a.new_table[e] = p >= used && p < a.pages && in_use(p) ? target(p) : p;
     }
   }
-  share(L, used - kept, [&](int move, int layer, int piece) KV_AI {
-    copy(L, layer, piece, uniform(select<true>(sums, ranges, bits, kept + move)), uniform(select<false>(sums, ranges, bits, move)), L.page / 16);
-  });
+  int src = 0, dst = 0;
+  share(L, used - kept, [&](int move) KV_AI {
+    src = uniform(select<true>(sums, ranges, bits, kept + move)), dst = uniform(select<false>(sums, ranges, bits, move));
+  }, [&](int layer, int piece) KV_AI { copy(L, layer, piece, src, dst, L.page / 16); });
 }
 
 long ranges_of(long pages) { return (pages + RANGE - 1) / RANGE; }

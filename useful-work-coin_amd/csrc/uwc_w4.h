@@ -84,5 +84,6 @@ __device__ __forceinline__ void w4_store(const W4Args& a, int m, int n, f4v v) {
   }
 }
 
-// The kernel for many rows (uwc_w4_gemm.hip).
+// The kernel for many rows (uwc_w4_gemm.hip), and about how many us it takes.
+float w4_gemm_us(const W4Args& a, bool gated);
 int w4_gemm(const char* fn, const W4Args& a, int dtype, bool gated, hipStream_t stream);

@@ -144,6 +144,16 @@ int rows(const char* fn, const W4Args& a, hipStream_t stream) {
   return uwc_launch_status(fn);
 }
 
+// About how many us the kernel above takes past 16 rows: `waves` of a workgroup take a unit each at a time, which lasts `one` us or, where
+// the workgroups wait for each other's loads, one for every `many` of them.
+// Against the tiles in LDS, K = 14016: 69 x 500 17 us (41 there), 128 x 1024 40 (43), 333 x 500 65 (45); K = 2048: 24 x 1024 5.0 (9.8),
+// 333 x 500 10.6 (10.0), 333 x 1024 18 (10).
+float few_rows_us(const W4Args& a, int tiles_of_x, int waves, float one, float many) {
+  const long units = (a.K + 255) / 256, groups = ((long)a.M + 16 * tiles_of_x - 1) / (16 * tiles_of_x) * (((long)a.F + 15) / 16);
+  const float each = groups / many;
+  return 2.9f + (units + waves - 1) / waves * (each > one ? each : one);
+}
+
 // More tiles of weights to a workgroup share the loads of x, which take longer than the codes from about four rows on (64 lines of
 // memory an instruction against 16); fewer, and more waves to a tile, keep all compute units at work. us, weights from HBM:
 //   gated, tiles x waves    2 x 4   4 x 4   2 x 8        linear                  1 x 8   2 x 8   4 x 4
@@ -152,11 +162,13 @@ int rows(const char* fn, const W4Args& a, hipStream_t stream) {
 //   1 x 6144 x 2048           6.5     7.6     6.8        8 x 28672 x 4096         32.1    25.5    20.5
 template <class T>
 int run(const char* fn, const W4Args& a, bool gated, hipStream_t stream) {
-  if (gated) return a.M > 4 ? rows<T, 1, 4, 4, true>(fn, a, stream) : rows<T, 1, 2, 4, true>(fn, a, stream);
-  if (a.M > 16) return rows<T, 2, 1, 8, false>(fn, a, stream);
-  if (a.F >= 16384) return rows<T, 1, 4, 4, false>(fn, a, stream);
-  if (a.F >= 6144) return rows<T, 1, 2, 8, false>(fn, a, stream);
-  return rows<T, 1, 1, 8, false>(fn, a, stream);
+  if (gated) return a.M > 4 && a.M <= 16 ? rows<T, 1, 4, 4, true>(fn, a, stream) : rows<T, 1, 2, 4, true>(fn, a, stream);
+  if (a.M <= 16) {
+    if (a.F >= 16384) return rows<T, 1, 4, 4, false>(fn, a, stream);
+    if (a.F >= 6144) return rows<T, 1, 2, 8, false>(fn, a, stream);
+    return rows<T, 1, 1, 8, false>(fn, a, stream);
+  }
+  return few_rows_us(a, 1, 8, 2, 85) <= few_rows_us(a, 2, 8, 3.2f, 50) ? rows<T, 1, 1, 8, false>(fn, a, stream) : rows<T, 2, 1, 8, false>(fn, a, stream);
 }
 
 int call(const char* fn, const W4Args& a, int dtype, bool gated, hipStream_t stream) {
@@ -168,9 +180,10 @@ int call(const char* fn, const W4Args& a, int dtype, bool gated, hipStream_t str
   if (a.x_stride > 1 << 22) return uwc_fail("%s: rows of x are %ld elements apart, more than 2^22", fn, a.x_stride);
   if (a.x_stride < 0 || a.x_stride % 8 || (((uintptr_t)a.x | (uintptr_t)a.codes) & 15) || ((uintptr_t)a.y & 7))
     return uwc_fail("%s: rows of x and codes must be 16-byte aligned, y 8-byte aligned", fn);
-  // the tiles in LDS from 17 rows on (24 x 6144 x 2048, gated: 13.8 us here, 11.7 there), of fewer weights from 33
-  // (24 x 4096 x 4096: 11.5 here, 16.5 there)
-  if (a.M > (gated || a.F > 8192 ? 16 : 32)) return w4_gemm(fn, a, dtype, gated, stream);
+  if (a.M > 16) {
+    const float one = few_rows_us(a, 1, gated ? 4 : 8, gated ? 1.6f : 2, gated ? 150 : 85), two = gated ? one : few_rows_us(a, 2, 8, 3.2f, 50);
+    if (w4_gemm_us(a, gated) < (one < two ? one : two)) return w4_gemm(fn, a, dtype, gated, stream);
+  }
   return dtype == UWC_W4_BF16 ? run<__bf16>(fn, a, gated, stream) : run<_Float16>(fn, a, gated, stream);
 }
 

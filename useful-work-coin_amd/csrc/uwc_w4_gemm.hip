@@ -252,24 +252,24 @@ int launch(const char* fn, const W4Args& a, hipStream_t stream) {
   return uwc_launch_status(fn);
 }
 
-// us that a round of tiles, one to a compute unit, spends on a step of a group: of one tile alone, and with all units at work (power, L2).
-// Measured over K = 4096 at 64 to 2048 rows of 4096 weights, and at 8192 rows; whole calls come within 15% of what they say
-// (512 x 4096 x 4096: 78, 52, 36, 26 and 34 us in the forms' order; 1024: 79, 55, 43, 53, 64; 2048: 86, 73, 86, 100, 125).
+// us of a round of tiles, one to a compute unit: to begin and end, and a step of a group with one tile alone at work and with all units
+// (power, L2). Measured over K = 2048 to 14336; calls of 64 to 2048 rows of 4096 weights, K = 4096, take within 10% of what this says:
+// 512 rows 78, 52, 36, 26 and 34 us in the forms' order; 1024 79, 55, 42, 52, 64; 2048 86, 64, 86, 100, 125.
 struct Form {
   int BM, rows, KG;
-  float alone, full;
+  float fixed, alone, full;
 };
-const Form forms[] = {{256, 256, 1, 1.19f, 1.6f}, {128, 256, 1, 0.8f, 1.15f}, {128, 128, 2, 1.03f, 1.34f}, {64, 128, 2, 0.69f, 0.78f}, {64, 64, 4, 1.05f, 0.97f}};
+const Form forms[] = {{256, 256, 1, 6, 1.09f, 1.55f}, {128, 256, 1, 7, 0.69f, 0.95f}, {128, 128, 2, 7, 0.8f, 1.1f}, {64, 128, 2, 6.5f, 0.47f, 0.62f},
+                      {64, 64, 4, 4.2f, 0.7f, 0.75f}};
 
-int choose(const W4Args& a, bool gated) {
+int choose(const W4Args& a, bool gated, float& least) {
   const long cus = uwc_cu_count(), steps = (a.K + 63) / 64;
   int best = 0;
-  float least = 0;
   for (int f = 0; f < 5; f++) {
     const Form& F = forms[f];
     const long out = F.rows / (gated ? 2 : 1), tiles = (((long)a.M + F.BM - 1) / F.BM) * ((a.F + out - 1) / out), rest = tiles % cus;
-    const float rounds = tiles / cus * F.full + (rest ? F.alone + (F.full - F.alone) * rest / cus : 0);
-    const float us = rounds * ((steps + 4 * F.KG - 1) / (4 * F.KG) * 4);
+    const float times = (steps + 4 * F.KG - 1) / (4 * F.KG) * 4;
+    const float us = tiles / cus * (F.fixed + times * F.full) + (rest ? F.fixed + times * (F.alone + (F.full - F.alone) * rest / cus) : 0);
     if (!f || us < least) best = f, least = us;
   }
   return best;
@@ -277,7 +277,8 @@ int choose(const W4Args& a, bool gated) {
 
 template <class T, bool GATED>
 int run(const char* fn, const W4Args& a, hipStream_t stream) {
-  switch (choose(a, GATED)) {
+  float us;
+  switch (choose(a, GATED, us)) {
     case 0: return launch<T, 1, 4, 2, 4, GATED>(fn, a, stream);
     case 1: return launch<T, 1, 2, 4, 2, GATED>(fn, a, stream);
     case 2: return launch<T, 2, 2, 2, 2, GATED>(fn, a, stream);
@@ -287,6 +288,12 @@ int run(const char* fn, const W4Args& a, hipStream_t stream) {
 }
 
 }  // namespace
+
+float w4_gemm_us(const W4Args& a, bool gated) {
+  float us;
+  choose(a, gated, us);
+  return us;
+}
 
 int w4_gemm(const char* fn, const W4Args& a, int dtype, bool gated, hipStream_t stream) {
   if (dtype == UWC_W4_BF16) return gated ? run<__bf16, true>(fn, a, stream) : run<__bf16, false>(fn, a, stream);
