@@ -468,7 +468,7 @@ int uwc_kv_read(const int8_t* k, const int8_t* v, const float* ks, const float* 
 
 /* Pages of a cache that sequences share. refs (int32, pages): how many hold a page, rows of the table and others; one
  * with none is free. caches: a HOST array of 4 * layers device pointers, k, v, ks and vs of each layer, all of the same shape;
- * every layer uses the same pages. At most 8192 rows, 2^22 pages. New tables (R or B rows of `width` entries, dense), lengths and
+ * every layer uses the same pages. At most 4096 rows, 2^21 pages, 2^31 entries of a table. New tables (R or B rows of `width` entries, dense), lengths and
  * counts are outputs of their own and overlap no input; the caches change in place. scratch: uwc_kv_pages_scratch_bytes(pages, R) bytes
  * (compact: R = 0), 16-byte aligned, no contents kept between calls. Entries outside [0, pages) are pages that are not
  * there: they are kept as they are and counted nowhere. */

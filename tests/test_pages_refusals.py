@@ -17,7 +17,7 @@ def i(*s, dt=torch.int32):
 @pytest.mark.parametrize("change,msg", [
     (dict(caches=[]), "no caches"), (dict(caches=[cpu(), cpu(pages=5)]), "one shape"), (dict(caches=[cpu(), cpu(hd=32)]), "one shape"),
     (dict(caches=[(i(2), i(2), i(2), i(2))]), "unpack"), (dict(table=i(2, 3, dt=torch.int64)), "page table"), (dict(table=i(3)), "page table"),
-    (dict(table=i(8193, 1), lens=i(8193)), "8193 rows"), (dict(refs=i(3)), "refs must be"), (dict(refs=i(4, dt=torch.int64)), "refs must be"),
+    (dict(table=i(4097, 1), lens=i(4097)), "4097 rows"), (dict(refs=i(3)), "refs must be"), (dict(refs=i(4, dt=torch.int64)), "refs must be"),
     ({}, "must be on a GPU"),
 ])
 def test_both_refuse(change, msg):
@@ -54,9 +54,9 @@ def call(name, caches=(FAKE,) * 8, **change):
 
 @pytest.mark.parametrize("change,msg", [
     (dict(layers=-1), "layers"), (dict(caches=(FAKE, FAKE, None, FAKE)), "null cache"), (dict(caches=(ODD, FAKE, FAKE, FAKE)), "aligned"),
-    (dict(caches=(FAKE, ODD, FAKE, FAKE)), "aligned"), (dict(pages=0), "pages"), (dict(pages=(1 << 22) + 1), "pages"), (dict(Hkv=0), "Hkv"),
+    (dict(caches=(FAKE, ODD, FAKE, FAKE)), "aligned"), (dict(pages=0), "pages"), (dict(pages=(1 << 21) + 1), "pages"), (dict(Hkv=0), "Hkv"),
     (dict(Hkv=65536), "Hkv"), (dict(page=24), "page 24"), (dict(hd=96), "head_dim"), (dict(width=-1), "bad width"), (dict(B=-1), "rows"),
-    (dict(B=8193), "rows"), (dict(stride=-1), "bad width"), (dict(table=None), "null"), (dict(refs=None), "null"),
+    (dict(B=4097), "rows"), (dict(width=1 << 22, B=1000), "2^31"), (dict(stride=-1), "bad width"), (dict(table=None), "null"), (dict(refs=None), "null"),
     (dict(scratch=None), "null"), (dict(bytes=100), "scratch"), (dict(scratch=ODD), "scratch"), (dict(new_table=None), "null"),
     (dict(new_refs=None), "null"),
 ])
@@ -67,7 +67,7 @@ def test_the_library_refuses(change, msg):
 
 
 @pytest.mark.parametrize("change,msg", [
-    (dict(R=-1), "rows"), (dict(R=8193), "rows"), (dict(room=-1), "room"), (dict(lens=None), "null"), (dict(parents=None), "null"),
+    (dict(R=-1), "rows"), (dict(R=4097), "rows"), (dict(room=-1), "room"), (dict(lens=None), "null"), (dict(parents=None), "null"),
     (dict(new_lens=None), "null"), (dict(missing=None), "null"), (dict(width=1 << 28), "2^31"),
 ])
 def test_fork_of_the_library_refuses(change, msg):

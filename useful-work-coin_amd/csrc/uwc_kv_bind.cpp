@@ -217,7 +217,7 @@ PyObject* fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!L.ok) return none();
   const int64_t B = table->size(0), width = table->size(1), R = parents->size(0);
   const at::Tensor *lens = L.ints(a[2], B), *refs = L.ints(a[3], c.pages);
-  if (!L.ok || !current(L) || B > 8192 || R > 8192 || width > I32MAX) return none();
+  if (!L.ok || !current(L) || B > 4096 || R > 4096 || width > I32MAX) return none();
   const long long room = PyLong_AsLongLong(a[5]);
   const hipStream_t stream = stream_of(a[6]);
   if (PyErr_Occurred()) return nullptr;
@@ -245,7 +245,7 @@ PyObject* compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t B = table->size(0), width = table->size(1);
   const hipStream_t stream = stream_of(a[3]);
   if (PyErr_Occurred()) return nullptr;
-  if (B > 8192 || width > I32MAX) return none();
+  if (B > 4096 || width > I32MAX) return none();
   const auto opt = refs->options();
   at::Tensor table_ = at::empty({B, width}, opt), refs_ = at::empty({c.pages}, opt);
   const uint64_t need = lib_pages_bytes(c.pages, 0);

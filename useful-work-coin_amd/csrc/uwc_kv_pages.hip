@@ -17,7 +17,7 @@
 namespace {
 
 constexpr int RANGE = 1024, WORDS = RANGE / 64;  // pages, words of 64 bits of a range
-constexpr int ROWS = 8192, RANGES = 4096;        // most rows and ranges of a call
+constexpr int ROWS = 4096, RANGES = 2048;        // most rows and ranges of a call: 32 KB of LDS, four workgroups to a unit
 constexpr int LAYERS = 64;                       // layers of a launch
 constexpr int UNITS = 2048;                      // 16-byte units of a piece
 
@@ -224,13 +224,12 @@ __global__ __launch_bounds__(256) void fork_plan_kernel(ForkArgs a, int ranges) 
     for (int r = t; r < a.B; r += 256)
       if (children[r] != 1) list[atomicAdd(&listed, 1)] = (unsigned short)r;
     __syncthreads();
-    const long entries = (long)listed * a.width;
-    for (long e0 = t; e0 < entries; e0 += 256 * 8) {
+    const u32 entries = (u32)listed * a.width;
+    for (u32 e0 = t; e0 < entries; e0 += 256 * 8) {
       int p[8], c[8];
 #pragma unroll
       for (int k = 0; k < 8; k++) {
-        const long e = e0 + 256 * k < entries ? e0 + 256 * k : entries - 1;
-        const u32 at = (u32)(e / a.width), j = (u32)(e - (long)at * a.width);
+        const u32 e = e0 + 256 * k < entries ? e0 + 256 * k : entries - 1, at = e / a.width, j = e % a.width;
         const int r = list[at];
         p[k] = a.table[r * a.stride + j];
         c[k] = children[r] ? (int)j < length(r) / a.page ? children[r] - 1 : 0 : -1;
@@ -338,14 +337,13 @@ __global__ __launch_bounds__(256) void compact_finish_kernel(CompactArgs a, Laye
   if (first_launch) {
     auto in_use = [&](int p) KV_AI { return bits[p / 64] >> (p % 64) & 1; };
     auto target = [&](int p) KV_AI { return select<false>(sums, ranges, bits, rank_of(sums, bits, p) - kept); };
-    const long me = blockIdx.x * 256L + threadIdx.x, step = gridDim.x * 256L;
-    for (long p = me; p < a.pages; p += step) {
-      const bool u = in_use((int)p);
-      if (u) a.new_refs[p < used ? p : target((int)p)] = a.refs[p];
+    const int me = blockIdx.x * 256 + threadIdx.x, step = gridDim.x * 256;
+    for (int p = me; p < a.pages; p += step) {
+      if (in_use(p)) a.new_refs[p < used ? p : target(p)] = a.refs[p];
       if (p >= used) a.new_refs[p] = 0;
     }
-    for (long e = me; e < (long)a.B * a.width; e += step) {
-      const int p = a.table[e / a.width * a.stride + e % a.width];
+    for (u32 e = me; e < (u32)a.B * a.width; e += step) {
+      const int p = a.table[(long)(e / a.width) * a.stride + e % a.width];
       a.new_table[e] = p >= used && p < a.pages && in_use(p) ? target(p) : p;
     }
   }
@@ -372,6 +370,7 @@ int check(const char* fn, int layers, void* const* caches, int64_t pages, int pa
   if (hd != 32 && hd != 64 && hd != 128) return uwc_fail("%s: head_dim %d not in {32, 64, 128}", fn, hd);
   if (width < 0 || B < 0 || B > ROWS || R < 0 || R > ROWS || stride < 0)
     return uwc_fail("%s: bad width=%d, rows %d and %d (at most %d)", fn, width, B, R, ROWS);
+  if ((long)(B > R ? B : R) * width > 0x7fffffff) return uwc_fail("%s: a table of %d rows of %d entries, more than 2^31", fn, B > R ? B : R, width);
   if ((B && width && !table) || !refs || !scratch) return uwc_fail("%s: null arguments", fn);
   if (bytes < uwc_kv_pages_scratch_bytes(pages, R) || ((uintptr_t)scratch & 15)) return uwc_fail("%s: the scratch is too small or not 16-byte aligned", fn);
   for (int i = 0; i < 4 * layers; i++) {
@@ -398,7 +397,7 @@ int by_layers(const char* fn, int layers, void* const* caches, int Hkv, int hd, 
 }
 
 // Workgroups of the second launch: as many as there can be jobs, up to what the compute units hold at once, which then take several
-// each (fork: 64 KB of LDS, two to a unit; four rounds of them, each finding its rows' ranks, took 10.5 us where nothing is copied).
+// each (fork: four to a unit; four rounds of them, each finding its rows' ranks, took 10.5 us where nothing is copied).
 unsigned grid_of(int to_a_unit, long jobs, long rows) {
   const long most = (long)to_a_unit * uwc_cu_count(), n = jobs > rows ? jobs : rows;
   return (unsigned)(n < 1 ? 1 : n < most ? n : most);
@@ -428,7 +427,7 @@ extern "C" int uwc_kv_fork(int layers, void* const* caches, int64_t pages, int p
   hipLaunchKernelGGL(fork_plan_kernel, dim3(ranges + R), dim3(256), 0, stream, a, ranges);
   if (int st = uwc_launch_status(fn)) return st;
   return by_layers(fn, layers, caches, Hkv, hd, page, [&](const Layers& L, bool first) {
-    hipLaunchKernelGGL(fork_finish_kernel, dim3(grid_of(2, R * pieces_on_host(Hkv, page, hd) * L.n, R)), dim3(256), 0, stream, a, L, ranges, first);
+    hipLaunchKernelGGL(fork_finish_kernel, dim3(grid_of(4, R * pieces_on_host(Hkv, page, hd) * L.n, R)), dim3(256), 0, stream, a, L, ranges, first);
   });
 }
 

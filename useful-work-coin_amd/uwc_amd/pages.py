@@ -27,7 +27,7 @@ import torch
 
 from . import _lib, kv
 
-ROWS = 8192
+ROWS = 4096
 _I32MAX = 2 ** 31 - 1
 
 
