@@ -248,3 +248,31 @@ def test_the_long_way_gives_the_same(dev, monkeypatch):
     short = run()
     monkeypatch.setattr(_lib, "_KV", _lib._LongWay)
     assert all(torch.equal(a, b) for a, b in zip(short, run()))
+
+
+def test_two_streams_at_once(dev):
+    """Calls on two streams overlap: each has its own workspace."""
+    from uwc_amd import pages as P, w4
+    import w4_reference as W
+    page = 32
+    rng = random.Random(21)
+    states = [R.state(rng, page, 40, 300, 4, spare=60) for _ in range(2)]
+    sets = [caches(4, s[3], 2, 64, page, i, dev) for i, s in enumerate(states)]
+    parents = [[rng.randrange(-1, 40) for _ in range(60)] for _ in range(2)]
+    inputs = [(ints(s[0], dev), ints(s[1], dev), ints(s[2], dev), ints(p, dev)) for s, p in zip(states, parents)]
+    g = torch.Generator().manual_seed(2)
+    codes, scales = (x.to(dev) for x in W.weight(512, 1024, g))
+    xs = [torch.randn((m, 1024), generator=g).bfloat16().to(dev) for m in (3, 400)]
+    want = [w4.linear(x, codes, scales) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append((P.fork(sets[i], *inputs[i], room=5), w4.linear(xs[i], codes, scales)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        wt, wl, wr, wm, _ = R.fork(states[i][0], states[i][1], states[i][2], parents[i], 5, page)
+        for (t, n, r, m), y in got[i]:
+            assert t.tolist() == wt and n.tolist() == wl and r.tolist() == wr and m.tolist() == [wm] and torch.equal(y, want[i])

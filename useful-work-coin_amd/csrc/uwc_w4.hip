@@ -1,5 +1,8 @@
-// Linears with 4-bit weights for few rows: the weights are streamed once per 16 to 64 rows, straight from memory into
+// Linears with 4-bit weights for few rows: the weights are streamed once per 16 or 32 rows, straight from memory into
 // the registers that the matrix instructions read.
+//
+// Bytes bound it, or at few of them a launch and the latency of its loads: one row of 2 x 14336 x 4096, gated, 17.3 us (62 MB, 3.6 TB/s;
+// 10.2 at the rate of a streaming read), one of 2048 x 2048 3.7 us.
 #include "uwc_w4.h"
 
 namespace {
