@@ -11,6 +11,11 @@ BF, HF = torch.bfloat16, torch.float16
 SHAPES = [(1, 1, 32), (1, 16, 64), (1, 257, 2048), (2, 33, 96), (3, 100, 4096), (7, 515, 160), (16, 64, 256), (17, 48, 1024), (32, 1000, 416),
           (33, 130, 2080), (64, 96, 512), (65, 257, 320), (100, 514, 1024), (128, 256, 2048), (200, 100, 128), (257, 300, 544), (300, 1111, 256),
           (513, 260, 96), (1000, 1030, 1056), (2049, 520, 160), (1030, 4100, 640), (4097, 1026, 384)]
+# every form that the rules choose: the tiles of 256 x 256 to 64 x 64 with one, two and four groups of waves, and of few rows
+# those for many weights
+FORMS = [(4096, 4096, 160), (4001, 4040, 224), (2048, 4096, 160), (2001, 4090, 96), (1024, 4096, 4096), (1000, 4090, 4064), (512, 4096, 2048),
+         (333, 4096, 4096), (500, 4001, 2080), (64, 4096, 1024), (60, 4001, 1056), (5, 16400, 96), (3, 6200, 160), (16, 20000, 544), (2, 9300, 288),
+         (40, 300, 9056)]
 
 
 def rows(M, K, g, dtype, dev):
@@ -18,7 +23,7 @@ def rows(M, K, g, dtype, dev):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
-@pytest.mark.parametrize("M,N,K", SHAPES)
+@pytest.mark.parametrize("M,N,K", SHAPES + FORMS)
 def test_linear(dev, M, N, K, dtype):
     from uwc_amd import w4
     g = torch.Generator().manual_seed(M * 7 + N + K)
@@ -33,7 +38,7 @@ def test_linear(dev, M, N, K, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
-@pytest.mark.parametrize("M,F,K", [(M, (N + 1) // 2, K) for M, N, K in SHAPES])
+@pytest.mark.parametrize("M,F,K", [(M, (N + 1) // 2, K) for M, N, K in SHAPES + FORMS])
 def test_gated(dev, M, F, K, dtype):
     from uwc_amd import w4
     g = torch.Generator().manual_seed(M * 5 + F + K)

@@ -147,14 +147,14 @@ int rows(const char* fn, const W4Args& a, hipStream_t stream) {
   return uwc_launch_status(fn);
 }
 
-// About how many us the kernel above takes past 16 rows: `waves` of a workgroup take a unit each at a time, which lasts `one` us or, where
+// About how many us the kernel above takes past 16 rows: the eight waves of a workgroup take a unit each at a time, which lasts `one` us or, where
 // the workgroups wait for each other's loads, one for every `many` of them.
 // Against the tiles in LDS, K = 14016: 69 x 500 17 us (41 there), 128 x 1024 40 (43), 333 x 500 65 (45); K = 2048: 24 x 1024 5.0 (9.8),
 // 333 x 500 10.6 (10.0), 333 x 1024 18 (10).
-float few_rows_us(const W4Args& a, int tiles_of_x, int waves, float one, float many) {
+float few_rows_us(const W4Args& a, int tiles_of_x, float one, float many) {
   const long units = (a.K + 255) / 256, groups = ((long)a.M + 16 * tiles_of_x - 1) / (16 * tiles_of_x) * (((long)a.F + 15) / 16);
   const float each = groups / many;
-  return 2.9f + (units + waves - 1) / waves * (each > one ? each : one);
+  return 2.9f + (units + 7) / 8 * (each > one ? each : one);
 }
 
 // More tiles of weights to a workgroup share the loads of x, which take longer than the codes from about four rows on (64 lines of
@@ -163,15 +163,22 @@ float few_rows_us(const W4Args& a, int tiles_of_x, int waves, float one, float m
 //   1 x 14336 x 4096         18.2    19.4    19.8        1 x 4096 x 14336         13.2    19.4    50.2
 //   16 x 14336 x 4096        40.1    25.2    39.9        13 x 6144 x 4096         12.3     8.9    12.8
 //   1 x 6144 x 2048           6.5     7.6     6.8        8 x 28672 x 4096         32.1    25.5    20.5
+//   1 x 2048 x 8192          14.6             10.3       (16 waves to a tile: within 3% of 8, 1 x 4096 x 14336 12.6)
+//   1 x 203 x 11104          17.0             11.2
+//   16 x 4096 x 4096                  15.3    11.5
+//   16 x 6144 x 4096                  15.7    19.3
 template <class T>
 int run(const char* fn, const W4Args& a, bool gated, hipStream_t stream) {
-  if (gated) return a.M > 4 && a.M <= 16 ? rows<T, 1, 4, 4, true>(fn, a, stream) : rows<T, 1, 2, 4, true>(fn, a, stream);
+  if (gated) {
+    if (a.M > 16 || a.F <= 4608) return rows<T, 1, 2, 8, true>(fn, a, stream);
+    return a.M > 4 ? rows<T, 1, 4, 4, true>(fn, a, stream) : rows<T, 1, 2, 4, true>(fn, a, stream);
+  }
   if (a.M <= 16) {
     if (a.F >= 16384) return rows<T, 1, 4, 4, false>(fn, a, stream);
     if (a.F >= 6144) return rows<T, 1, 2, 8, false>(fn, a, stream);
     return rows<T, 1, 1, 8, false>(fn, a, stream);
   }
-  return few_rows_us(a, 1, 8, 2, 85) <= few_rows_us(a, 2, 8, 3.2f, 50) ? rows<T, 1, 1, 8, false>(fn, a, stream) : rows<T, 2, 1, 8, false>(fn, a, stream);
+  return few_rows_us(a, 1, 2, 85) <= few_rows_us(a, 2, 3.2f, 50) ? rows<T, 1, 1, 8, false>(fn, a, stream) : rows<T, 2, 1, 8, false>(fn, a, stream);
 }
 
 int call(const char* fn, const W4Args& a, int dtype, bool gated, hipStream_t stream) {
@@ -184,7 +191,7 @@ int call(const char* fn, const W4Args& a, int dtype, bool gated, hipStream_t str
   if (a.x_stride < 0 || a.x_stride % 8 || (((uintptr_t)a.x | (uintptr_t)a.codes) & 15) || ((uintptr_t)a.y & 7))
     return uwc_fail("%s: rows of x and codes must be 16-byte aligned, y 8-byte aligned", fn);
   if (a.M > 16) {
-    const float one = few_rows_us(a, 1, gated ? 4 : 8, gated ? 1.6f : 2, gated ? 150 : 85), two = gated ? one : few_rows_us(a, 2, 8, 3.2f, 50);
+    const float one = few_rows_us(a, 1, gated ? 3 : 2, gated ? 75 : 85), two = gated ? one : few_rows_us(a, 2, 3.2f, 50);
     if (w4_gemm_us(a, gated) < (one < two ? one : two)) return w4_gemm(fn, a, dtype, gated, stream);
   }
   return dtype == UWC_W4_BF16 ? run<__bf16>(fn, a, gated, stream) : run<_Float16>(fn, a, gated, stream);
