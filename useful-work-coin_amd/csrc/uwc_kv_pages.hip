@@ -11,8 +11,8 @@
 // Two launches each. The first writes one bit a page (free, or in use), sums of them over 1024 pages, and what each row
 // needs; the second's workgroups find a page by its rank from those sums, each for itself, copy, and write
 // tables and counts. Nothing goes by the order in which workgroups run. Copies are bound by HBM, in pieces of at most 32 KB to a
-// workgroup (1.76 GB in 375 us, 4.7 TB/s, what a copy reaches here; one prompt into 32 rows, 171 MB in 34); the rest is a chain of short
-// dependent loads (256 rows of 252 entries, nothing copied: 11 + 5 us).
+// workgroup (1.76 GB in 375 us, 4.7 TB/s, what a copy reaches here; one prompt into 32 rows, 171 MB in 32); the rest is a chain of short
+// dependent loads (256 rows of 252 entries, nothing copied: 9 + 5 us).
 #include "uwc_kv.h"
 
 namespace {
