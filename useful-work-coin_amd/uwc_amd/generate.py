@@ -205,20 +205,35 @@ class PagedGenerator:
         self.free.extend(reversed(prefix.pages))
 
     def resize(self, pages: int):
-        """Makes the caches hold `pages` pages, at least those that kept prefixes have; their pages move to the front first."""
-        used, now = sum(len(p.pages) for p in self.kept), self.caches[0][0].shape[0]
-        if pages < max(1, used):
-            raise AssertionError(f"resize: {pages} pages, of which {used} are in use")
-        if pages < now and used:
+        """Makes the caches hold `pages` pages, at least those that kept prefixes have; their pages move to the front first.
+        Where memory runs out on the way, a larger pool stays as it was, and a smaller one has its `pages` pages but still the memory
+        of the layers that were not reached, which another call gives back."""
+        held, now = [i for p in self.kept for i in p.pages], self.caches[0][0].shape[0]
+        if pages < max(1, len(held)):
+            raise AssertionError(f"resize: {pages} pages, of which {len(held)} are in use")
+        if pages < now and held:
             refs = torch.zeros(now, dtype=torch.int32)
-            refs[[i for p in self.kept for i in p.pages]] = 1
+            refs[held] = 1
             # one row holds them all: a page is named once
-            table, _ = pool.compact(self.caches, self._ints([[i for p in self.kept for i in p.pages]]), refs.to(self.dev))
-            moved = iter(table[0].tolist())
+            table, _ = pool.compact(self.caches, self._ints([held]), refs.to(self.dev))
+            held = table[0].tolist()
+            moved = iter(held)
             for p in self.kept:
                 p.pages = [next(moved) for _ in p.pages]
-        for i, c in enumerate(self.caches):  # a layer at a time: the old and the new one of one layer alone exist together
-            self.caches[i] = tuple(torch.cat([x, x.new_zeros((pages - now, *x.shape[1:]))]) if pages > now else x[:pages].clone() for x in c)
-            del c
-        taken = {i for p in self.kept for i in p.pages}
-        self.free = [i for i in range(pages) if i not in taken]
+        # A layer at a time: the old and the new cache of one layer alone exist together. What is free and how many pages the layers
+        # have are in step before memory is asked for, and after it is refused
+        if pages <= now:
+            self.caches = [tuple(x[:pages] for x in c) for c in self.caches]
+            self._free_all_but(held, pages)
+        try:
+            for i in range(len(self.caches)):
+                self.caches[i] = tuple(torch.cat([x, x.new_zeros((pages - now, *x.shape[1:]))]) if pages > now else x.clone()
+                                       for x in self.caches[i])
+        except BaseException:
+            self.caches = [tuple(x[:now] for x in c) for c in self.caches]
+            raise
+        self._free_all_but(held, pages)
+
+    def _free_all_but(self, held, pages: int):
+        held = set(held)
+        self.free = [i for i in range(pages) if i not in held]
