@@ -291,13 +291,28 @@ class FourBitMLP(nn.Module):
         return self.down(w4.gated(x, self.gate_up.codes, self.gate_up.scales))
 
 
+def _check_4bit(name: str, lin: nn.Linear):
+    w = lin.weight.detach()
+    if w.dtype not in (torch.bfloat16, torch.float16):
+        raise AssertionError(f"convert_4bit: {name} must be bfloat16 or float16, got {w.dtype}")
+    if w.dim() != 2 or w.shape[1] == 0 or w.shape[1] % w4.GROUP:
+        raise AssertionError(f"convert_4bit: {name} must have a positive multiple of {w4.GROUP} inputs, got weights {tuple(w.shape)}")
+    if w.numel() and not torch.isfinite(torch.stack(torch.aminmax(w))).all():
+        raise AssertionError(f"convert_4bit: {name} must have finite weights")
+
+
 def convert_4bit(model, device, lm_head: bool = False) -> list[nn.Module]:
     """Replace the linears of a Hugging Face Qwen3 or Llama model (a CausalLM or the bare model), in bfloat16 or float16, by
     FourBitLinears, q/k/v fused and each feed-forward block a FourBitMLP; returns them per layer (qkv, o, feed-forward), then
-    the lm_head where it is asked for. The weights are rounded to 4 bits as they are, without calibration."""
+    the lm_head where it is asked for. The weights are rounded to 4 bits as they are, without calibration. A model that cannot
+    be converted is refused before anything in it is replaced."""
     decoder = getattr(model, "model", model)
-    for layer in decoder.layers:  # before anything is replaced
+    for i, layer in enumerate(decoder.layers):
         FourBitMLP.check(layer.mlp)
+        for name in ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj", "self_attn.o_proj", "mlp.gate_proj", "mlp.up_proj", "mlp.down_proj"):
+            _check_4bit(f"layers.{i}.{name}", layer.get_submodule(name))
+    if lm_head and hasattr(model, "lm_head"):
+        _check_4bit("lm_head", model.lm_head)
     out = []
     for layer in decoder.layers:
         att = layer.self_attn
