@@ -95,6 +95,8 @@ def _call(fn, x, codes, scales):
     if x.dtype not in _TYPES or x.device != codes.device or x.dim() < 1 or x.shape[-1] != K:
         raise AssertionError(f"{fn}: x must be bfloat16 or float16 (..., {K}) on the weight's device, got {x.dtype} "
                              f"{tuple(x.shape)} on {x.device}")
+    if max(N, K, x.numel() // K) > kv._I32MAX:
+        raise AssertionError(f"{fn}: rows, outputs and K must be below 2^31, got {x.numel() // K}, {N} and {K}")
     if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 16:
         raise AssertionError(f"{fn}: codes and scales must be contiguous, codes 16-byte aligned")
     if x.device.type != "cuda":
