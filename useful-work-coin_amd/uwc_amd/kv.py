@@ -92,6 +92,8 @@ def _table(fn, table, dev):
     if table.dtype != torch.int32 or table.dim() != 2 or table.device != dev:
         raise AssertionError(f"{fn}: the page table must be int32 (B, width) on the cache's GPU, got {table.dtype} "
                              f"{tuple(table.shape)} on {table.device}")
+    if max(table.shape) > _I32MAX:
+        raise AssertionError(f"{fn}: a page table of {tuple(table.shape)} entries, 2^31 or more on a side")
     return table if table.shape[1] < 2 or table.stride(1) == 1 else table.contiguous()
 
 
@@ -99,6 +101,8 @@ def _rows16(fn, name, x, dev):
     """A 16-bit tensor whose rows are dense and 16-byte aligned: x itself where it is so already."""
     if x.dtype not in _TYPES or x.device != dev:
         raise AssertionError(f"{fn}: {name} must be bfloat16 or float16 on the cache's GPU, got {x.dtype} on {x.device}")
+    if x.shape[0] > _I32MAX:
+        raise AssertionError(f"{fn}: {name} has {x.shape[0]} rows, 2^31 or more")
     dense = x.stride(-1) == 1 and (x.dim() == 2 or x.stride(1) == x.shape[2])
     return x if dense and x.stride(0) >= 0 and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0 else x.clone(
         memory_format=torch.contiguous_format)
