@@ -42,9 +42,9 @@ def _require(ok, msg):
 
 
 def quantize(w: torch.Tensor):
-    """(codes, scales) of a matrix w (N, K), K a multiple of 32, of finite numbers: a group's scale is the power of two that brings
-    its largest magnitude into [4, 8) (an all-zero group's is 2^-127), each weight the nearest value, ties to the code
-    with a zero low bit, 6 where it is larger."""
+    """(codes, scales) of a matrix w (N, K), K a multiple of 32, of finite numbers within float32: a group's scale is the power of
+    two, at least 2^-127, that brings its largest magnitude into [4, 8) (an all-zero group's is 2^-127), each weight the nearest
+    value, ties to the code with a zero low bit, 6 where it is larger."""
     _require(w.dim() == 2 and w.is_floating_point() and w.shape[1] % GROUP == 0 and w.shape[1] > 0,
              f"w4.quantize: w must be a floating-point (N, K) with K a positive multiple of {GROUP}, got {w.dtype} {tuple(w.shape)}")
     N, K = w.shape
@@ -53,9 +53,10 @@ def quantize(w: torch.Tensor):
     powers = _powers(w.device)
     step = max(1, (1 << 25) // K)  # rows at a time: an lm_head never needs a whole fp32 copy
     for n in range(0, N, step):
-        x = w[n:n + step].detach().float().unflatten(1, (-1, GROUP))
+        x = w[n:n + step].detach()
+        x = (x if x.dtype == torch.float64 else x.float()).unflatten(1, (-1, GROUP))
         top = x.abs().amax(-1, keepdim=True)
-        _require(bool(torch.isfinite(top).all()), "w4.quantize: w has infinities or NaN")
+        _require(bool(torch.isfinite(top.float()).all()), "w4.quantize: w has infinities or NaN")
         e = (torch.frexp(top).exponent - 3).clamp(min=-127)  # top = m 2^(e + 3), m in [0.5, 1)
         e = torch.where(top > 0, e, -127)
         y = x.double().abs() / powers[(e + 127).long()]  # below 8
