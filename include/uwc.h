@@ -500,7 +500,8 @@ int uwc_kv_compact(int layers, void* const* caches, int64_t pages, int page, int
  * w[n, k] = value(code) 2^(scale[n, k / 32] - 127), value = 0, 0.5, 1, 1.5, 2, 3, 4, 6, negated where the code's top
  * bit is set; a scale of 255 makes its row's outputs NaN. Rows are dense, K a positive multiple of 32, at most 2^22. x: M rows,
  * x_stride (at most 2^22) elements apart; x, its rows and codes 16-byte aligned, y (dense, x's type) 8-byte aligned. Sums are fp32,
- * rounded once; bf16 rows meet the weights exactly, fp16 rows the weights rounded to fp16 (exact for scales from 103 to 140). */
+ * rounded once; bf16 rows meet weights below 2^128 (any of scales up to 252) exactly, fp16 rows the weights rounded to fp16 (exact for
+ * scales from 104 to 140). Weights past that, and for fp16 rows of 65520 and more, are infinite, their outputs infinite or NaN. */
 #define UWC_W4_BF16 0
 #define UWC_W4_FP16 1
 

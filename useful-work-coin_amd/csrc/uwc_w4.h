@@ -5,7 +5,8 @@
 // with value(code) = 0, 0.5, 1, 1.5, 2, 3, 4, 6 and the same negated: the fp4 elements and power-of-two group scales
 // of the OCP microscaling format. A row's codes are K / 2 bytes, the weight of the lower k in a byte's low half;
 // its scales K / 32 bytes. value times a power of two is exact in bf16 (two bits of 8), so the matrix instructions take the
-// true weights. fp16 has less range: weights of float16 rows are rounded to it (exact for scales from 103 to 140).
+// true weights, as long as those are below 2^128 (any of scales up to 252; larger ones are infinite). fp16 has less range: weights of float16
+// rows are rounded to it (exact for scales from 104 to 140; 65520 and more is infinite).
 #pragma once
 #include "uwc_common.h"
 

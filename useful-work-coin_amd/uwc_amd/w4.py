@@ -12,9 +12,9 @@ column 2 i + 1 in the high half, scales uint8 (N, K / 32), one for each group of
   linear    x W^T (+ bias)
   gated     silu(x G^T) * (x U^T): both projections, the activation and the product of a feed-forward block in one kernel
 
-Rows x are bfloat16 or float16, sums fp32, rounded once to x's type. bfloat16 rows meet the weights exactly; for
-float16 rows the weights are rounded to float16 (exact for scales from 103 to 140; of larger ones those past 65504 are infinite,
-and outputs that they meet infinite or not a number).
+Rows x are bfloat16 or float16, sums fp32, rounded once to x's type. bfloat16 rows meet weights below 2^128 exactly, which all of
+scales up to 252 are; for float16 rows the weights are rounded to float16 (exact for scales from 104 to 140). Weights past
+those ranges (2^128, and for float16 65520) are infinite, and the outputs that they meet infinite or not a number.
 A scale of 255 is not a number: its row's outputs are NaN. Nothing is recorded for autograd.
 
 Everything runs on torch's current HIP stream; buffers are torch tensors on the caller's GPU. Arguments of the usual form
