@@ -487,7 +487,8 @@ int uwc_kv_fork(int layers, void* const* caches, int64_t pages, int page, int Hk
                 uint64_t scratch_bytes, hipStream_t stream);
 
 /* With n pages held: those from n on move, in their order, to the free ones below n, in every layer; the new table and
- * counts name them there, and no page from n on is held. */
+ * counts name them there, and no page from n on is held. Holders that are no rows of the table learn their pages' new numbers
+ * only as rows of the call. */
 int uwc_kv_compact(int layers, void* const* caches, int64_t pages, int page, int Hkv, int hd, const int32_t* table,
                    int64_t table_stride, int width, int B, const int32_t* refs, int32_t* new_table, int32_t* new_refs,
                    void* scratch, uint64_t scratch_bytes, hipStream_t stream);

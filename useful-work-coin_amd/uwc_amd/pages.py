@@ -92,7 +92,10 @@ def fork(caches, table: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, pa
 
 def compact(caches, table: torch.Tensor, refs: torch.Tensor):
     """(table, refs) after the pages in use, n of them, have moved to the first n places of the pool, in every layer: those
-    from n on, in their order, to the free ones before n; the others stay. A pool may then be cut to its first n pages."""
+    from n on, in their order, to the free ones before n; the others stay. A pool may then be cut to its first n pages.
+
+    All pages in use move, but only the table is renamed: who holds pages without being a row of it gives them as a row of this
+    call, of their numbers alone, and reads the new ones there."""
     r = _lib.kv().compact(caches, table, refs, kv._stream())
     if r is not None:
         return r if type(r) is not int else _lib.fail("uwc_kv_compact", r)
