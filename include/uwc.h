@@ -502,7 +502,8 @@ int uwc_kv_compact(int layers, void* const* caches, int64_t pages, int page, int
  * bit is set; a scale of 255 makes its row's outputs NaN. Rows are dense, K a positive multiple of 32, at most 2^22. x: M rows,
  * x_stride (at most 2^22) elements apart; x, its rows and codes 16-byte aligned, y (dense, x's type) 8-byte aligned. Sums are fp32,
  * rounded once; bf16 rows meet weights below 2^128 (any of scales up to 252) exactly, fp16 rows the weights rounded to fp16 (exact for
- * scales from 104 to 140). Weights past that, and for fp16 rows of 65520 and more, are infinite, their outputs infinite or NaN. */
+ * scales from 104 to 140). Weights past that, and for fp16 rows of 65520 and more, are infinite, their outputs infinite or NaN.
+ * The order of a row's sums depends on M, N and K alone: a call repeats its bits, a row in a call of another M may differ in the last ones. */
 #define UWC_W4_BF16 0
 #define UWC_W4_FP16 1
 

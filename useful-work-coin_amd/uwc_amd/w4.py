@@ -17,6 +17,9 @@ scales up to 252 are; for float16 rows the weights are rounded to float16 (exact
 those ranges (2^128, and for float16 65520) are infinite, and the outputs that they meet infinite or not a number.
 A scale of 255 is not a number: its row's outputs are NaN. Nothing is recorded for autograd.
 
+The same call gives the same bits every time. Which kernel runs, and in how many parts it sums, goes by the number of rows (and N and
+K): the same row among others may differ in the last bits, unlike in the framework's integer linears.
+
 Everything runs on torch's current HIP stream; buffers are torch tensors on the caller's GPU. Arguments of the usual form
 take the short way of uwc_amd.kv.
 """
