@@ -187,7 +187,8 @@ class _SharedOutput:
     from the cache while the input is the same tensor object at the same version (the cache
     holds the input itself, so a later tensor that reuses its address never matches); once
     every part has taken its slice the cache and the input are dropped, so no activation
-    outlives its layer."""
+    outlives its layer. Inference tensors (torch.inference_mode) have no version: nothing is kept of them,
+    each part is computed when it is asked for, alone where the linear can."""
 
     def __init__(self, ml: MinedLinear):
         self.ml = ml
@@ -197,6 +198,10 @@ class _SharedOutput:
         self._pending = 0
 
     def part(self, x: torch.Tensor, index: int) -> torch.Tensor:
+        if x.is_inference():
+            if hasattr(self.ml, "part"):
+                return self.ml.part(x, index)
+            return torch.split(self.ml(x), self.ml.splits, dim=-1)[index]
         if self._parts is None or self._x is not x or self._version != x._version:
             self._parts = torch.split(self.ml(x), self.ml.splits, dim=-1)
             self._x, self._version, self._pending = x, x._version, len(self._parts)
@@ -268,6 +273,12 @@ class FourBitLinear(nn.Module):
     @torch.compiler.disable
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return w4.linear(x, self.codes, self.scales, self.bias)
+
+    def part(self, x: torch.Tensor, index: int) -> torch.Tensor:
+        """What the fused layer number `index` gives."""
+        at = sum(self.splits[:index])
+        rows = slice(at, at + self.splits[index])
+        return w4.linear(x, self.codes[rows], self.scales[rows], None if self.bias is None else self.bias[rows])
 
 
 class FourBitMLP(nn.Module):
