@@ -2,7 +2,7 @@
 // the matrix instructions (a conversion of two takes 4 cycles beside the 32 of a product of 32 x 32 x 16, of which two share it).
 //
 // 8192 x 4096 x 14336 in 706 to 780 us by box (1230 to 1360 TFLOP/s, 82% of the library's bf16 product of the same size), the matrix units busy
-// 54% of the time; 2048 x 2 x 14336 x 4096, gated, in 397 to 431; 333 x 4096 x 4096 in 24, where few tiles and a barrier a step bound it.
+// 74% of the cycles (54% of those that the full clock would have); 2048 x 2 x 14336 x 4096, gated, in 397 to 431; 333 x 4096 x 4096 in 24, where few tiles and a barrier a step bound it.
 #include "uwc_w4.h"
 
 namespace {
